@@ -451,6 +451,65 @@ int32_t inf_paged_decode_attention_resident(inf_ctx* ctx, const float* q, const 
 int32_t inf_linearize_paged(inf_ctx* ctx, const void* pool_f16, const inf_kv_pool* shape,
                             const inf_page_table* table, int32_t tokens, void* out_f16);
 
+/* ---- ragged batches: every sequence brings its own number of new tokens ------------------------------------------- */
+/* One step of a continuously batched server holds prompt chunks, drafts and decodes together.  Its request lengths live
+ * on the GPU, so that a captured step can be replayed with other lengths.  The step is three calls:
+ *   inf_device_index_append     pages for the new tokens, and each token's position and slot
+ *   inf_rope_append_gqa_ragged  norm + RoPE of the projections, keys and values stored to the slots
+ *   inf_gqa_attention_ragged    attention of each sequence's new tokens over its pages
+ * and inf_device_index_truncate when drafts are rejected or a sequence ends.  All device pointers; nothing is copied to
+ * the host.  What the host cannot check is checked by the kernels and reported by inf_flush.
+ * (The reference serves one sequence at a time and has no counterpart.) */
+
+/* inf_paged_index on the GPU: caller-owned int32 arrays.  Slots of `pages` below ceil(lens[b] / page_size) hold page ids;
+ * the free list is a stack, free_pages[0 .. *free_count).  num_pages * page_size and max_pages * page_size must fit 31
+ * bits.  One call at a time may work on an index. */
+typedef struct inf_device_index {
+    int32_t* pages;      /* [max_seqs][max_pages] */
+    int32_t* lens;       /* [max_seqs] tokens cached */
+    int32_t* free_pages; /* [num_pages] */
+    int32_t* free_count; /* [1] */
+    int32_t num_pages, page_size, max_seqs, max_pages;
+} inf_device_index;
+/* Everything free: slots -1, lengths 0, and a stack that hands out pages 0, 1, 2, ... like a new inf_paged_index. */
+int32_t inf_device_index_reset(inf_ctx* ctx, const inf_device_index* index);
+/* new_tokens[b] >= 0 more tokens for every sequence, pages taken from the stack sequence by sequence as
+ * inf_paged_index_append would.  Written: past_lens [max_seqs] (lengths before the step: the `lens` of the page table
+ * that inf_gqa_attention_ragged takes), q_starts [max_seqs + 1] (first row of each sequence in the step's tensors; the
+ * last entry is the number of rows), positions and slots [max_tokens] (slot = page id * page_size + offset; -1 in rows
+ * behind the last token).  A step that does not fit -- more rows than max_tokens, a sequence longer than its table row,
+ * more pages than are free -- is refused as a whole: the index stays as it is, the outputs describe a step without
+ * tokens, and inf_flush reports it. */
+int32_t inf_device_index_append(inf_ctx* ctx, const inf_device_index* index, const int32_t* new_tokens, int32_t max_tokens,
+                                int32_t* past_lens, int32_t* q_starts, int32_t* positions, int32_t* slots);
+/* Cuts sequence b to keep_lens[b] tokens (0 releases it, a negative value leaves it alone) and pushes its pages back, the
+ * last sequence's last page first: a truncate to the lengths before an append restores the free list exactly.  A length
+ * above the present one refuses the whole call (inf_flush). */
+int32_t inf_device_index_truncate(inf_ctx* ctx, const inf_device_index* index, const int32_t* keep_lens);
+
+/* inf_rope_append_gqa with a position and a slot per token: q [tokens][q_heads][128], k / v [tokens][kv_heads][128] in
+ * in_dtype, heads contiguous, tokens q_stride / k_stride / v_stride elements apart (parts of one projection's rows need
+ * no copy).  q_out_f16 [tokens][q_heads][128] receives the roped queries.  Rows with a negative position are padding and
+ * touch nothing.  A slot outside the pool is reported and its key and value dropped; slots of one call must differ.
+ * Angles are exact for every 31-bit position.  Without a rope table rows are stored as they are (no norm either). */
+int32_t inf_rope_append_gqa_ragged(inf_ctx* ctx, const void* q, const void* k, const void* v, int64_t q_stride,
+                                   int64_t k_stride, int64_t v_stride, int32_t in_dtype, const float* q_norm_weight,
+                                   const float* k_norm_weight, float eps, const inf_rope_table* rope,
+                                   const inf_kv_pool* pool, const int32_t* positions, const int32_t* slots,
+                                   int32_t tokens, int32_t q_heads, void* q_out_f16);
+
+/* Causal attention of each sequence's new tokens over its pages: q fp16 [tokens][q_heads][128], rows q_starts[b] ..
+ * q_starts[b + 1] belong to sequence b (none is fine; q_starts must not decrease), table->lens[b] = keys cached BEFORE
+ * them, and their own keys and values have been appended at lens[b] onwards.  Row t sees keys [max(0, p + 1 - window), p],
+ * p = lens[b] + t.  gate f32 [tokens][q_heads] (optional) applies softplus(gate); scale <= 0 means 1/sqrt(128); out
+ * [tokens][q_heads][128] in out_dtype.  Rows from q_starts[batch] on are left as they were.  Up to 128 query heads per KV
+ * head (INF_UNSUPPORTED beyond).  A sequence whose rows or length do not fit is skipped and reported, a page id outside
+ * the pool is reported and its keys read as zeros.  Keys and values of visible tokens must be finite; pool slots behind a
+ * sequence's last token may hold anything. */
+int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, const inf_kv_pool* pool, const inf_page_table* table,
+                                 const int32_t* q_starts, int32_t tokens, int32_t q_heads, int32_t sliding_window,
+                                 const float* gate, float scale, void* out, int32_t out_dtype);
+
 /* ---- multi-GPU: the one collective of the path ------------------------------------------------------ */
 /* Head-sharded prefill / MLA leaves every rank with [tokens, heads/N, dim]; the output is all-gathered over
  * NCCL (NVLink / NVSwitch) on the context's stream.  (The reference is single-device; no counterpart.)

@@ -65,6 +65,25 @@ class PageTable:
     host_lens: Optional[torch.Tensor] = None
 
 
+@dataclass
+class DeviceIndex:
+    """Page bookkeeping of many sequences on the GPU (the device twin of paged.PagedIndex); int32 tensors."""
+    pages: torch.Tensor       # [max_seqs, max_pages]
+    lens: torch.Tensor        # [max_seqs] tokens cached
+    free_pages: torch.Tensor  # [num_pages], a stack
+    free_count: torch.Tensor  # [1]
+    desc: L.DeviceIndex
+
+
+@dataclass
+class RaggedBatch:
+    """One step's layout, written by device_index_append; int32 tensors on the GPU."""
+    past_lens: torch.Tensor  # [max_seqs] tokens cached before the step
+    q_starts: torch.Tensor   # [max_seqs + 1] first row of each sequence
+    positions: torch.Tensor  # [max_tokens], -1 behind the last token
+    slots: torch.Tensor      # [max_tokens] page id * page_size + offset, -1 behind the last token
+
+
 class CudaBackend:
     def __init__(self, device: int = 0, stream: Optional[torch.cuda.Stream] = None):
         if not torch.cuda.is_available():
@@ -234,6 +253,26 @@ class CudaBackend:
         self._check(self._lib.inf_download(self._ctx, C.c_void_p(out.data_ptr()), _ptr(dev), dev.numel() * 4))
         return out
 
+    def _mine(self, what: str, dtype, *tensors, contiguous: bool = True):
+        """The arguments of one call: on this context's GPU, of one dtype, contiguous unless the call takes strides."""
+        for t in tensors:
+            if t is None:
+                continue
+            if t.device != self.device:
+                raise InfernoError(L.INF_E_ARG, f"{what}: tensor on {t.device}, the context is on {self.device}")
+            if t.dtype != dtype:
+                raise InfernoError(L.INF_E_DTYPE, f"{what}: expected {dtype}, got {t.dtype}")
+            if contiguous and not t.is_contiguous():
+                raise InfernoError(L.INF_E_ARG, f"{what}: tensor must be contiguous")
+
+    def _new(self, shape, dtype) -> torch.Tensor:
+        """Memory for an output that the library's stream writes: from that stream's pool, so that no other stream's
+        pending work still uses it."""
+        if self.stream.cuda_stream == torch.cuda.current_stream(self.device).cuda_stream:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(self.stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
     # ------------------------------------------------------------------ descriptors
     def prepare_rope_table(self, inv_freq, rotary_dim: int, attention_factor: float) -> L.RopeTable:  # backend.rs:1227
         host = torch.as_tensor(inv_freq, dtype=torch.float32).contiguous()
@@ -251,6 +290,15 @@ class CudaBackend:
         k = torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=torch.float16, device=self.device)
         v = torch.zeros_like(k)
         return KvPool(k, v, L.KvPool(k.data_ptr(), v.data_ptr(), num_pages, page_size, kv_heads, head_dim))
+
+    def kv_pool(self, k: torch.Tensor, v: torch.Tensor) -> KvPool:
+        """Existing fp16 tensors [num_pages, kv_heads, page_size, 128] as a pool."""
+        self._mine("kv_pool", torch.float16, k, v)
+        if k.dim() != 4 or k.shape != v.shape or k.shape[3] != 128:
+            raise InfernoError(L.INF_E_SHAPE, f"kv_pool: expected [pages, heads, page_size, 128] twice, got {tuple(k.shape)}, {tuple(v.shape)}")
+        if k.shape[2] % 16:
+            raise InfernoError(L.INF_E_CACHE, f"page_size must be a positive multiple of 16, got {k.shape[2]}")
+        return KvPool(k, v, L.KvPool(k.data_ptr(), v.data_ptr(), k.shape[0], k.shape[2], k.shape[1], k.shape[3]))
 
     def prepare_kv_pool_fp8(self, num_pages: int, page_size: int, kv_heads: int, key_scale: float, value_scale: float,
                             head_dim: int = 128) -> KvPoolFp8:
@@ -285,6 +333,120 @@ class CudaBackend:
         desc = L.PageTable(dp.data_ptr(), dl.data_ptr(), dp.shape[0], dp.shape[1],
                            hp.data_ptr() if hp is not None else None, hl.data_ptr() if hl is not None else None)
         return PageTable(dp, dl, desc, hp, hl)
+
+    # ------------------------------------------------------------------ ragged batches
+    # One step of a continuously batched server, prompt chunks, drafts and decodes together: device_index_append lays it
+    # out, rope_append_gqa_ragged stores its keys and values, gqa_attention_ragged attends, device_index_truncate drops
+    # what was rejected.  Lengths stay on the GPU, so a captured step can be replayed with others.
+    def prepare_device_index(self, num_pages: int, page_size: int, max_seqs: int, max_pages: int) -> DeviceIndex:
+        """A new index: every page free, every sequence empty."""
+        if min(num_pages, page_size, max_seqs, max_pages) <= 0:
+            raise InfernoError(L.INF_E_CACHE, "device index sizes must be positive")
+        index = self.device_index(self._new((max_seqs, max_pages), torch.int32), self._new((max_seqs,), torch.int32),
+                                  self._new((num_pages,), torch.int32), self._new((1,), torch.int32), page_size)
+        self.device_index_reset(index)
+        return index
+
+    def device_index(self, pages, lens, free_pages, free_count, page_size: int) -> DeviceIndex:
+        """Existing int32 tensors as an index (inf_device_index says what they hold)."""
+        self._mine("device_index", torch.int32, pages, lens, free_pages, free_count)
+        if pages.dim() != 2 or lens.shape != pages.shape[:1] or free_pages.dim() != 1 or free_count.numel() != 1:
+            raise InfernoError(L.INF_E_SHAPE, "device_index: expected pages [seqs, max_pages], lens [seqs], a stack and its count")
+        return DeviceIndex(pages, lens, free_pages, free_count,
+                           L.DeviceIndex(pages.data_ptr(), lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+                                         free_pages.numel(), page_size, pages.shape[0], pages.shape[1]))
+
+    def device_index_reset(self, index: DeviceIndex):
+        self._check(self._lib.inf_device_index_reset(self._ctx, C.byref(index.desc)))
+
+    def prepare_ragged_batch(self, max_seqs: int, max_tokens: int) -> RaggedBatch:
+        """Buffers for the layout of steps of up to max_tokens new tokens."""
+        if min(max_seqs, max_tokens) <= 0:
+            raise InfernoError(L.INF_E_SHAPE, "ragged batch sizes must be positive")
+        return RaggedBatch(*(self._new((n,), torch.int32) for n in (max_seqs, max_seqs + 1, max_tokens, max_tokens)))
+
+    def device_index_append(self, index: DeviceIndex, new_tokens: torch.Tensor, batch: RaggedBatch) -> RaggedBatch:
+        """Reserve new_tokens[b] more slots per sequence; the step's layout goes into `batch`.  A step that does not fit
+        changes nothing, describes no tokens and is reported by device_flush."""
+        self._mine("device_index_append", torch.int32, new_tokens, batch.past_lens, batch.q_starts, batch.positions, batch.slots)
+        seqs = index.desc.max_seqs
+        if new_tokens.shape != (seqs,) or batch.past_lens.shape != (seqs,) or batch.q_starts.shape != (seqs + 1,) \
+                or batch.positions.shape != batch.slots.shape:
+            raise InfernoError(L.INF_E_SHAPE, f"device_index_append: the index has {seqs} sequences, got {tuple(new_tokens.shape)} lengths")
+        self._check(self._lib.inf_device_index_append(
+            self._ctx, C.byref(index.desc), new_tokens.data_ptr(), batch.positions.numel(), batch.past_lens.data_ptr(),
+            batch.q_starts.data_ptr(), batch.positions.data_ptr(), batch.slots.data_ptr()))
+        return batch
+
+    def device_index_truncate(self, index: DeviceIndex, keep_lens: torch.Tensor):
+        """Cut sequence b to keep_lens[b] tokens (0 releases it, negative leaves it alone); its pages become free."""
+        self._mine("device_index_truncate", torch.int32, keep_lens)
+        if keep_lens.shape != (index.desc.max_seqs,):
+            raise InfernoError(L.INF_E_SHAPE, f"device_index_truncate: the index has {index.desc.max_seqs} sequences, got {tuple(keep_lens.shape)} lengths")
+        self._check(self._lib.inf_device_index_truncate(self._ctx, C.byref(index.desc), keep_lens.data_ptr()))
+
+    def rope_append_gqa_ragged(self, q, k, v, rope, pool: KvPool, positions, slots, q_norm=None, k_norm=None, eps=1e-6,
+                               out=None):
+        """rope_append_gqa with a position and a slot per token: q [T, Hq, 128], k / v [T, Hkv, 128] (f32 or fp16; they may
+        be parts of one projection's rows, heads contiguous).  Returns roped q (fp16); padding rows (position -1) of it
+        and of the pools are not touched."""
+        if q.dtype not in (torch.float32, torch.float16):
+            raise InfernoError(L.INF_E_DTYPE, "rope_append_gqa_ragged: q/k/v must share dtype f32 or f16")
+        what, d, hkv = "rope_append_gqa_ragged", pool.desc.head_dim, pool.desc.kv_heads
+        self._mine(what, q.dtype, q, k, v, contiguous=False)
+        self._mine(what, torch.int32, positions, slots)
+        self._mine(what, torch.float32, q_norm, k_norm)
+        T, Hq = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+        if q.shape != (T, Hq, d) or k.shape != (T, hkv, d) or v.shape != (T, hkv, d) or positions.shape != (T,) or slots.shape != (T,):
+            raise InfernoError(L.INF_E_SHAPE, f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, positions "
+                                              f"{tuple(positions.shape)}, slots {tuple(slots.shape)} do not fit {hkv} KV heads of {d}")
+        if any(w is not None and w.shape != (d,) for w in (q_norm, k_norm)):
+            raise InfernoError(L.INF_E_SHAPE, f"{what}: norm weights must have {d} values")
+        for t in (q, k, v):
+            if T and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != d)):
+                raise InfernoError(L.INF_E_ARG, f"{what}: the heads of a token must be contiguous")
+        if out is None:
+            out = self._new((T, Hq, d), torch.float16)
+        else:
+            self._mine(what, torch.float16, out)
+            if out.shape != (T, Hq, d):
+                raise InfernoError(L.INF_E_SHAPE, f"{what}: out must be {(T, Hq, d)}, got {tuple(out.shape)}")
+        # a single token's stride is never used: any tensor may stand there
+        qs, ks, vs = ((t.stride(0) if T > 1 else t.shape[1] * d) for t in (q, k, v))
+        self._check(self._lib.inf_rope_append_gqa_ragged(
+            self._ctx, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs,
+            L.DTYPE_F32 if q.dtype == torch.float32 else L.DTYPE_F16, q_norm.data_ptr() if q_norm is not None else None,
+            k_norm.data_ptr() if k_norm is not None else None, eps, C.byref(rope) if rope is not None else None,
+            C.byref(pool.desc), positions.data_ptr(), slots.data_ptr(), T, Hq, out.data_ptr()))
+        return out
+
+    def gqa_attention_ragged(self, q_f16, pool: KvPool, table: PageTable, q_starts, sliding_window: int = 0, gate=None,
+                             scale: float = 0.0, out_dtype=torch.float16, out=None):
+        """Causal attention of each sequence's new tokens over its pages: q [T, Hq, 128], rows q_starts[b] .. q_starts[b + 1]
+        belong to sequence b, table.lens counts the keys cached before them.  Rows behind the last sequence's keep
+        what `out` holds."""
+        what = "gqa_attention_ragged"
+        self._mine(what, torch.float16, q_f16)
+        self._mine(what, torch.int32, q_starts)
+        self._mine(what, torch.float32, gate)
+        if q_f16.dim() != 3 or q_f16.shape[2] != pool.desc.head_dim or q_starts.shape != (table.desc.batch + 1,):
+            raise InfernoError(L.INF_E_SHAPE, f"{what}: q {tuple(q_f16.shape)} and q_starts {tuple(q_starts.shape)} do not fit heads of "
+                                              f"{pool.desc.head_dim} and {table.desc.batch} sequences")
+        T, Hq, D = q_f16.shape
+        if gate is not None and gate.shape != (T, Hq):
+            raise InfernoError(L.INF_E_SHAPE, f"{what}: gate must be {(T, Hq)}, got {tuple(gate.shape)}")
+        if out is None:
+            out = self._new((T, Hq, D), out_dtype)
+        if out.shape != q_f16.shape:
+            raise InfernoError(L.INF_E_SHAPE, f"{what}: out must be {(T, Hq, D)}, got {tuple(out.shape)}")
+        if out.dtype not in (torch.float32, torch.float16):
+            raise InfernoError(L.INF_E_DTYPE, f"{what}: output dtype must be f32 or f16")
+        self._mine(what, out.dtype, out)
+        ok = self._check(self._lib.inf_gqa_attention_ragged(
+            self._ctx, q_f16.data_ptr(), C.byref(pool.desc), C.byref(table.desc), q_starts.data_ptr(), T, Hq, sliding_window,
+            gate.data_ptr() if gate is not None else None, scale, out.data_ptr(),
+            L.DTYPE_F32 if out.dtype == torch.float32 else L.DTYPE_F16))
+        return out if ok else None
 
     # ------------------------------------------------------------------ RoPE + append
     def qk_rms_norm_rope_device(self, x, norm_weight, eps, position_offset, table):  # backend.rs:1238

@@ -17,6 +17,7 @@
 #define INF_STATUS_BAD_PAGE 2      // a page id outside the pool was refused
 #define INF_STATUS_BAD_LEN 4       // a length that does not fit the page table or the size the launch was given
 #define INF_STATUS_BAD_SMEM 8      // the dynamic shared-memory base is not aligned as the tiles need
+#define INF_STATUS_NO_PAGES 16     // the free list holds fewer pages than a step needs, or more than the pool has
 
 typedef CUresult (*inf_tmap_encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                        const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -94,6 +95,29 @@ int inf_make_tmap_typed(inf_ctx* ctx, const void* base, uint32_t rank, const uin
     do {                   \
         if (!(ctx)) return INF_E_ARG; \
     } while (0)
+
+// Makes the context's GPU the current one for the scope of an entry point and puts the caller's back afterwards.
+struct inf_device_scope {
+    int before = -1;
+    bool switched = false;
+    explicit inf_device_scope(inf_ctx* ctx) {
+        if (cudaGetDevice(&before) == cudaSuccess && before != ctx->device) switched = cudaSetDevice(ctx->device) == cudaSuccess;
+    }
+    ~inf_device_scope() {
+        if (switched) cudaSetDevice(before);
+    }
+};
+
+// Runs the body of an entry point on the context's GPU; an exception of the host code (out of memory) becomes a status.
+template <typename F>
+int inf_entry(inf_ctx* ctx, F&& body) noexcept {
+    try {
+        inf_device_scope scope(ctx);
+        return body();
+    } catch (...) {
+        return INF_E_BACKEND;
+    }
+}
 
 #define INF_CUDA(ctx, call)                                                                              \
     do {                                                                                                 \

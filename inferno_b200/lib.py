@@ -55,6 +55,11 @@ class PageTable(C.Structure):
                 ("host_pages", C.c_void_p), ("host_lens", C.c_void_p)]
 
 
+class DeviceIndex(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("lens", C.c_void_p), ("free_pages", C.c_void_p), ("free_count", C.c_void_p),
+                ("num_pages", C.c_int32), ("page_size", C.c_int32), ("max_seqs", C.c_int32), ("max_pages", C.c_int32)]
+
+
 _P = C.c_void_p
 _I = C.c_int32
 _F = C.c_float
@@ -125,6 +130,12 @@ SIGNATURES = {
     "inf_q8_0_packed_heads_matvec": (_I, [_P, _P, _P, _I, _I, _I, _I, _P]),
     "inf_q8_0_absorbed_mla": (_I, [_P, _P, _P, _P, _P, _P, _P, C.POINTER(MlaPool), C.POINTER(PageTable), _I, _I, _I,
                                    _I, _I, _I, _P]),
+    "inf_device_index_reset": (_I, [_P, C.POINTER(DeviceIndex)]),
+    "inf_device_index_append": (_I, [_P, C.POINTER(DeviceIndex), _P, _I, _P, _P, _P, _P]),
+    "inf_device_index_truncate": (_I, [_P, C.POINTER(DeviceIndex), _P]),
+    "inf_rope_append_gqa_ragged": (_I, [_P, _P, _P, _P, _L, _L, _L, _I, _P, _P, _F, C.POINTER(RopeTable),
+                                        C.POINTER(KvPool), _P, _P, _I, _I, _P]),
+    "inf_gqa_attention_ragged": (_I, [_P, _P, C.POINTER(KvPool), C.POINTER(PageTable), _P, _I, _I, _I, _P, _F, _P, _I]),
     "inf_mla_prefill_causal": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _L, _P, _L, _L, _I, _I, _I, _I, _I, _F, _P, _L,
                                     _L, _I]),
     "inf_linearize_paged": (_I, [_P, _P, C.POINTER(KvPool), C.POINTER(PageTable), _I, _P]),
