@@ -158,6 +158,7 @@ int32_t inf_ctx_destroy(inf_ctx* ctx) {
         cudaEventDestroy(r.b);
     }
     if (ctx->workspace) cudaFree(ctx->workspace);
+    if (ctx->ragged_scratch) cudaFree(ctx->ragged_scratch);
     for (void* w : ctx->retired_workspaces) cudaFree(w);
     if (ctx->status) cudaFree(ctx->status);
     if (ctx->host_status) cudaFreeHost(ctx->host_status);

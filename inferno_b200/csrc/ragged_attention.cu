@@ -4,97 +4,800 @@
 // Row t of sequence b stands at p = past_b + t and sees the keys [max(0, p + 1 - window), p]:
 //     o = softplus(gate) * sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),   s_j = scale q . k_j,  m = max_j s_j
 // in one pass over the keys with a running maximum and sum.
+//
+// Work.  The G query heads of a KV head share its keys, so the rows of a KV head are packed: row = token * G + head, a
+// STREAM is up to 128 rows (Ts = 128 / G tokens), and an ITEM is (sequence, KV head, up to 2 Ts tokens): two streams that
+// read every 128-key tile together.  An item of one stream's tokens (decodes, drafts) has both streams on the same rows,
+// tile by tile in turn, and merges them at the end.
+//
+// One persistent CTA per SM.  The lengths are on the GPU, so the CTAs divide the work themselves: an item costs its keys
+// plus a fixed amount, the costs of all items stand in one line (sequence, KV head, tile of tokens), and CTA c takes the
+// c-th of equal parts of it.  Sums over a sequence's items have a closed form, so a scan over the batch and a binary
+// search find both ends.  A part's ends fall inside items, at tiles of keys; such an item's pieces leave (max, sum, row)
+// in scratch, and the CTA that finishes its last piece joins them in the order of the keys: nothing depends on timing.
+//
+// Twelve warps:
+//   warps 0-3, 4-7   softmax and epilogue of stream 0 / 1: thread = row = TMEM lane
+//   warp 8           walks the CTA's items, describes each in shared memory for the others, loads Q and the K ring (TMA)
+//   warp 9           issues S = Q K^T (SS, M128 N128 K16) into the ONE S buffer the streams share; a softmax warpgroup
+//                    copies its rows out at once, which frees the buffer for the other stream's next S
+//   warp 10          loads the V ring (TMA)
+//   warp 11          issues O += P V (TS: P packed fp16 in TMEM, V MN-major straight from its [key][dim] tile)
+// Rings and counters run on from item to item: the next item's K and V arrive while the last one's rows are written.
+// TMEM: S 128 columns, then per stream P 64 and O 128.  Shared memory: Q 2 x 32 KB, K 3 x 32 KB, V 2 x 32 KB.
 #include <cuda_fp16.h>
 #include <math.h>
 
 #include "common.cuh"
 #include "ptx.cuh"
+#include "ragged_parts.h"
 
 using namespace inf;
 
 namespace {
 
 constexpr int D = 128;
+constexpr int BM = 128, BN = RAGGED_TILE;
+constexpr int THREADS = 384;
+constexpr int KS = 3, VS = 2;          // tiles in the K and V rings
+constexpr int SR = 4;                  // rotation of the S barriers: a K slot is looked at up to KS - 1 tiles late
+constexpr int TILE_BYTES = BN * D * 2;  // also the bytes of a stream's Q
+constexpr int BLK_BYTES = BN * 128;    // [128 rows][64 columns] with the 128-byte swizzle
+constexpr int RING = 4;                // item descriptions in flight
 constexpr float M_INIT = -1.0e30f;
+constexpr float RESCALE_THRESHOLD = 8.0f;
+constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_STREAM = 128, STREAM_COLS = 192, COL_P = 0, COL_O = 64;
+
+struct Item {
+    int b, kvh, tok0, ntok;        // tokens [tok0, tok0 + ntok) of the step
+    int qpos0, kv_total, lowest;   // position of the first token, keys of the sequence, lowest key any row sees
+    int kt0, kt1;                  // key tiles of this piece; kt0 == kt1 ends the CTA's work
+    int pieces, ordinal, group;    // of an item cut over several CTAs: how many, which one, the CTA of the first
+};
+
+struct Shared {
+    uint64_t q_full[2], q_free[2], k_full[KS], v_full[VS];
+    uint64_t s_full[2][SR];   // S of a stream's tile is in TMEM; its K tile has been read if no other stream reads it
+    uint64_t s_free;          // the S buffer has been copied into registers
+    uint64_t p_full[2][2];    // keys 0-63 / 64-127 of a stream's P are in TMEM
+    uint64_t o_ready[2][2];   // PV of a stream's tile has retired; its V tile likewise
+    uint64_t item_full[RING], item_free[RING];
+    uint64_t q_dead;          // every S of an item of shared rows has retired: its Q tiles take stream 1's rows
+    uint64_t pair_bar[2], part_bar, flag_bar;  // those rows are there / have been read; pieces
+    uint32_t tmem;
+    int last_piece;
+    Item items[RING];
+    long long scan[THREADS / 32];
+    int end[4], begin[4];          // (sequence, KV head, tile of tokens, key tile)
+    int cut[2][3];                 // pieces, ordinal, group of the first and of the last item
+    float ml[BM][2];
+};
+
+constexpr int OFF_K = 2 * TILE_BYTES, OFF_V = OFF_K + KS * TILE_BYTES, OFF_SHARED = OFF_V + VS * TILE_BYTES;
+constexpr int SMEM_BYTES = OFF_SHARED + (int)sizeof(Shared);
+static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 
 struct RaggedParams {
-    const __half* q;
-    const __half *k, *v;
     const int *pages, *lens, *starts;
     int batch, max_pages, tokens, q_heads, kv_heads, group, page_size, num_pages, window;
+    int stream_tokens;  // Ts
+    int box_rows;       // keys of one TMA box
     float scale_log2;
     const float* gate;
     void* out;
     int out_f16;
+    float *part_acc, *part_ml;  // [2 grid][256] rows
+    int* counters;              // [grid], zero between launches
     int* status;
 };
 
 // log(1 + e^v): log1p, because 1 + e^v keeps nothing but 2^-24 of e^v, which is 1e-3 of it at v = -10.
 __device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
 
-// A sequence's rows and cached keys; false (and the status word) where they do not fit what the launch was given.
-__device__ __forceinline__ bool sequence_of(const RaggedParams& p, int b, int& start, int& n, int& past) {
-    start = p.starts[b];
-    n = p.starts[b + 1] - start;
-    past = p.lens[b];
-    if (n == 0) return false;
-    if (start < 0 || n < 0 || (long long)start + n > p.tokens || past < 0 || (long long)past + n > (long long)p.max_pages * p.page_size) {
-        atomicOr(p.status, INF_STATUS_BAD_LEN);
-        return false;
+// ---------------------------------------------------------------------------------------------- the line of work
+struct Seq {
+    int start, n, past;
+};
+
+// A sequence's rows and cached keys; n = 0 (and a status bit) where they do not fit what the launch was given.
+__device__ __forceinline__ Seq sequence_of(const RaggedParams& p, int b, int& bad) {
+    Seq s;
+    s.start = p.starts[b];
+    s.n = p.starts[b + 1];
+    s.past = p.lens[b];
+    const long long n = (long long)s.n - s.start;
+    s.n = (int)n;
+    if (n < 0 || (n > 0 && (s.start < 0 || s.start + n > p.tokens || s.past < 0 || s.past + n > (long long)p.max_pages * p.page_size))) {
+        bad = INF_STATUS_BAD_LEN;
+        s.n = 0;
+    }
+    return s;
+}
+
+template <typename T>
+__device__ __forceinline__ T block_sum_before(T v, T& before, T* s_warp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+    }
+    if (lane == 31) s_warp[warp] = inc;
+    __syncthreads();
+    T base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) base += s_warp[w];
+        total += s_warp[w];
+    }
+    before = base + inc - v;
+    return total;
+}
+
+// Where CTA c's part of the line begins and ends.  Returns false where it has none.
+__device__ __forceinline__ bool find_part(const RaggedParams& p, Shared& sh) {
+    const int tid = threadIdx.x, c = blockIdx.x;
+    const int per = (p.batch + THREADS - 1) / THREADS, b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+    int bad = 0;
+    long long mine = 0, before;
+    for (int b = b0; b < b1; ++b) {
+        const Seq s = sequence_of(p, b, bad);
+        mine += p.kv_heads * RaggedHead(s.n, s.past, 2 * p.stream_tokens, p.window).total();
+    }
+    if (bad && c == 0) atomicOr(p.status, bad);
+    if (tid == 0) {
+        sh.end[0] = p.batch;
+        sh.end[1] = sh.end[2] = sh.end[3] = 0;
+        sh.cut[1][0] = 1;
+    }
+    const long long total = block_sum_before(mine, before, sh.scan);
+    const int parts = ragged_parts(total, (int)gridDim.x);
+    if (c >= parts) return false;
+    const long long x[2] = {ragged_cut(total, parts, c), ragged_cut(total, parts, c + 1)};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        if (x[e] >= before && x[e] < before + mine) {
+            long long at = before;
+            for (int b = b0; b < b1; ++b) {
+                const Seq s = sequence_of(p, b, bad);
+                const RaggedHead h(s.n, s.past, 2 * p.stream_tokens, p.window);
+                const long long cost = p.kv_heads * h.total();
+                if (x[e] < at + cost) {
+                    int* out = e == 0 ? sh.begin : sh.end;
+                    out[0] = b;
+                    ragged_locate(h, at, x[e], total, parts, c, out + 1, sh.cut[e]);
+                    break;
+                }
+                at += cost;
+            }
+        }
     }
     return true;
 }
 
-// One warp per (token, query head): lane holds four of the 128 dims, keys one after the other.
-__global__ void __launch_bounds__(256)
-ragged_attention_kernel(RaggedParams p) {
-    inf_pdl_wait();
-    inf_pdl_release();
-    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    const int t = (int)(row / p.q_heads), h = (int)(row % p.q_heads);
-    if (t >= p.tokens) return;
-    int lo = 0, hi = p.batch;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.starts[mid] <= t)
-            lo = mid;
-        else
-            hi = mid;
+// ---------------------------------------------------------------------------------------------- the kernel
+// A bounded wait of a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
+// A role's view of the items: the next one's description, copied to registers.
+struct ItemReader {
+    int count = 0;
+    __device__ __forceinline__ bool next(Shared& sh, Item& it) {
+        const int slot = count % RING;
+        if (!warp_wait(&sh.item_full[slot], (uint32_t)(count / RING) & 1u)) return false;
+        it = sh.items[slot];
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.item_free[slot]);
+        ++count;
+        return true;
     }
-    int start, n, past;
-    if (!sequence_of(p, lo, start, n, past) || t < start || t >= start + n) return;
-    const int pos = past + t - start;
-    const int first = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
-    const uint2 qraw = reinterpret_cast<const uint2*>(p.q + row * D)[lane];
-    const float2 q0 = __half22float2(*reinterpret_cast<const __half2*>(&qraw.x)), q1 = __half22float2(*reinterpret_cast<const __half2*>(&qraw.y));
-    float m = M_INIT, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int key = first; key <= pos; ++key) {
-        const int page = p.pages[(long long)lo * p.max_pages + key / p.page_size];
-        if (page < 0 || page >= p.num_pages) {
-            if (lane == 0) atomicOr(p.status, INF_STATUS_BAD_PAGE);
-            continue;
+};
+
+// Both streams on the same rows, tiles in turn.
+__device__ __forceinline__ bool shares_rows(const RaggedParams& p, const Item& it) { return it.ntok <= p.stream_tokens; }
+
+// Who reads a tile last: (stream, that stream's count of tiles) of the last three tiles, so that a producer knows which
+// barrier says that a ring slot is free.  MMAs of one thread retire in order, so the last reader speaks for both.
+struct TileLog {
+    int cnt0 = 0, cnt1 = 0, back0 = 0, back1 = 0, back2 = 0;
+    __device__ __forceinline__ void add(bool shared_rows, int turn) {
+        back2 = back1;
+        back1 = back0;
+        if (shared_rows && turn == 0) {
+            back0 = cnt0++ << 1;
+        } else {
+            back0 = cnt1++ << 1 | 1;
+            if (!shared_rows) ++cnt0;
         }
-        const long long at = (((long long)page * p.kv_heads + h / p.group) * p.page_size + key % p.page_size) * D;
-        const uint2 kr = reinterpret_cast<const uint2*>(p.k + at)[lane], vr = reinterpret_cast<const uint2*>(p.v + at)[lane];
-        const float2 k0 = __half22float2(*reinterpret_cast<const __half2*>(&kr.x)), k1 = __half22float2(*reinterpret_cast<const __half2*>(&kr.y));
-        float s = q0.x * k0.x + q0.y * k0.y + q1.x * k1.x + q1.y * k1.y;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        s *= p.scale_log2;
-        const float m_new = fmaxf(m, s), alpha = ex2_approx(m - m_new), w = ex2_approx(s - m_new);
-        const float2 v0 = __half22float2(*reinterpret_cast<const __half2*>(&vr.x)), v1 = __half22float2(*reinterpret_cast<const __half2*>(&vr.y));
-        m = m_new;
-        l = l * alpha + w;
-        o[0] = o[0] * alpha + w * v0.x, o[1] = o[1] * alpha + w * v0.y;
-        o[2] = o[2] * alpha + w * v1.x, o[3] = o[3] * alpha + w * v1.y;
     }
-    float gain = l > 0.f ? 1.0f / l : 0.f;
-    if (p.gate) gain *= softplus(p.gate[row]);
-    if (p.out_f16)
-        reinterpret_cast<uint2*>((__half*)p.out + row * D)[lane] = make_uint2(pack_half2(o[0] * gain, o[1] * gain), pack_half2(o[2] * gain, o[3] * gain));
-    else
-        reinterpret_cast<float4*>((float*)p.out + row * D)[lane] = make_float4(o[0] * gain, o[1] * gain, o[2] * gain, o[3] * gain);
+};
+static_assert(KS == 3 && VS == 2, "back2 is the tile that a K slot held, back1 the tile that a V slot held");
+
+// Row coordinates of the TMA boxes of 128 / box_rows tiles at a time, one box per lane, the next group looked up ahead.
+struct PageWalk {
+    int per_tile, tiles;  // boxes per tile, tiles per group of 32 boxes
+    int group = -1, y = 0, ahead = 0;
+    __device__ __forceinline__ explicit PageWalk(const RaggedParams& p) : per_tile(BN / p.box_rows), tiles(32 / (BN / p.box_rows)) {}
+    __device__ __forceinline__ int lookup(const RaggedParams& p, const Item& it, int g, bool report) const {
+        const int token = (g * tiles * BN) + (int)(threadIdx.x & 31) * p.box_rows;
+        int row = p.num_pages * p.kv_heads * p.page_size;  // outside the tensor: zeros
+        // boxes wholly below the lowest visible key may lie in pages that were given back
+        if (token < it.kv_total && token / BN < it.kt1 && token + p.box_rows > it.lowest) {
+            const int page = p.pages[(long long)it.b * p.max_pages + token / p.page_size];
+            if (page >= 0 && page < p.num_pages)
+                row = (page * p.kv_heads + it.kvh) * p.page_size + token % p.page_size;
+            else if (report)
+                atomicOr(p.status, INF_STATUS_BAD_PAGE);
+        }
+        return row;
+    }
+    __device__ __forceinline__ void begin(const RaggedParams& p, const Item& it, bool report) {
+        group = it.kt0 / tiles;
+        y = lookup(p, it, group, report);
+        ahead = lookup(p, it, group + 1, report);
+    }
+    __device__ __forceinline__ void step_to(const RaggedParams& p, const Item& it, int kt, bool report) {
+        if (kt / tiles == group) return;
+        group = kt / tiles;
+        y = ahead;
+        ahead = lookup(p, it, group + 1, report);
+    }
+    // one [128 keys][128 dims] tile as two blocks of 64 columns; every lane issues its boxes
+    __device__ __forceinline__ void load(const CUtensorMap* tm, const RaggedParams& p, int kt, uint8_t* dst, uint64_t* bar) const {
+        const int lane = threadIdx.x & 31, box = lane >> 1, blk = lane & 1;
+        const int row = __shfl_sync(0xffffffffu, y, (kt % tiles) * per_tile + (box < per_tile ? box : 0));
+        if (lane == 0) mbar_arrive_expect_tx(bar, TILE_BYTES);
+        __syncwarp();
+        if (box < per_tile) tma_load_2d(dst + blk * BLK_BYTES + box * p.box_rows * 128, tm, blk * 64, row, bar);
+    }
+};
+
+__global__ void __launch_bounds__(THREADS, 1)
+ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, RaggedParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *sQ = smem, *sK = smem + OFF_K, *sV = smem + OFF_V;
+    Shared& sh = *reinterpret_cast<Shared*>(smem + OFF_SHARED);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool smem_ok = (smem_u32(smem) & 1023u) == 0;  // the swizzled tiles need a 1024-byte aligned base
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.q_full[i], 1);
+            mbar_init(&sh.q_free[i], 1);
+            for (int j = 0; j < SR; ++j) mbar_init(&sh.s_full[i][j], 1);
+            for (int j = 0; j < 2; ++j) mbar_init(&sh.p_full[i][j], 4);  // one arrival per warp: tcgen05.wait is warp-wide
+            for (int j = 0; j < 2; ++j) mbar_init(&sh.o_ready[i][j], 1);
+        }
+        for (int i = 0; i < KS; ++i) mbar_init(&sh.k_full[i], 1);
+        for (int i = 0; i < VS; ++i) mbar_init(&sh.v_full[i], 1);
+        mbar_init(&sh.s_free, 4);
+        for (int i = 0; i < RING; ++i) {
+            mbar_init(&sh.item_full[i], 1);
+            mbar_init(&sh.item_free[i], 11);  // every warp but the one that writes
+        }
+        mbar_init(&sh.q_dead, 1);
+        mbar_init(&sh.pair_bar[0], 4);
+        mbar_init(&sh.pair_bar[1], 4);
+        mbar_init(&sh.part_bar, 8);
+        mbar_init(&sh.flag_bar, 1);
+        mbar_fence_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(&sh.tmem, TMEM_COLS);
+        tmem_relinquish();
+    }
+    if (warp == 8 && lane == 0) {
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+    }
+    inf_pdl_wait();  // queries, appended rows, lengths and page table come from work earlier in the stream
+    inf_pdl_release();
+    const bool has_work = find_part(p, sh) && smem_ok;
+    if (!smem_ok && tid == 0) atomicOr(p.status, INF_STATUS_BAD_SMEM);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = sh.tmem;
+
+    if (!has_work) {
+        // nothing to do for this CTA
+    } else if (warp >= 8) {
+        setmaxnreg_dec<56>();
+        ItemReader reader;
+        Item it;
+        bool alive = true;
+        if (warp == 8) {
+            // ------------------------------------------------ items, Q and the K ring
+            int b = sh.begin[0], kvh = sh.begin[1], i = sh.begin[2], kt = sh.begin[3], bad = 0;
+            const int eb = sh.end[0], ekvh = sh.end[1], ei = sh.end[2], ekt = sh.end[3];
+            bool first = true;     // still in the item the part begins in
+            int items = 0, tiles = 0;
+            TileLog log;
+            int q_uses[2] = {0, 0};
+            int base = -32;
+            Seq s{0, 0, 0};
+            PageWalk walk(p);
+            while (alive) {
+                // ---- the sequence: metadata of 32 at a time, one per lane
+                if (b >= p.batch || b > eb) break;
+                if (b >= base + 32) {
+                    base = b;
+                    if (base + lane < p.batch)
+                        s = sequence_of(p, base + lane, bad);
+                    else
+                        s.n = 0;
+                }
+                const int n = __shfl_sync(0xffffffffu, s.n, b - base), past = __shfl_sync(0xffffffffu, s.past, b - base),
+                          start = __shfl_sync(0xffffffffu, s.start, b - base);
+                const RaggedHead h(n, past, 2 * p.stream_tokens, p.window);
+                if (i >= h.items) {
+                    i = 0;
+                    if (n == 0 || ++kvh >= p.kv_heads) {
+                        kvh = 0;
+                        ++b;
+                    }
+                    continue;
+                }
+                // ---- the item, and how much of it is this CTA's
+                const bool last = b == eb && kvh == ekvh && i == ei;
+                const bool past_end = b > eb || (b == eb && (kvh > ekvh || (kvh == ekvh && i > ei)));
+                if (past_end) break;
+                it.kt0 = first ? kt : h.first_tile(i);
+                it.kt1 = last ? ekt : h.end_tile(i);
+                const int* cut = first ? sh.cut[0] : sh.cut[1];
+                const bool cut_here = first || last;
+                it.pieces = cut_here ? cut[0] : 1;
+                it.ordinal = cut_here ? cut[1] : 0;
+                it.group = cut_here ? cut[2] : 0;
+                first = false;
+                it.b = b;
+                it.kvh = kvh;
+                it.tok0 = start + i * h.T;
+                it.ntok = min(h.T, n - i * h.T);
+                it.qpos0 = past + i * h.T;
+                it.kv_total = past + n;
+                it.lowest = h.lo(i);
+                ++i;
+                if (it.kt0 >= it.kt1) {
+                    if (last) break;
+                    continue;
+                }
+                // ---- tell the others
+                const int slot = items % RING;
+                if (items >= RING) alive = warp_wait(&sh.item_free[slot], (uint32_t)(items / RING - 1) & 1u);
+                if (!alive) break;
+                if (lane == 0) sh.items[slot] = it;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.item_full[slot]);
+                ++items;
+                // ---- Q: a stream's tile is free when its last S has retired (or its rows have been merged)
+                const bool shared_rows = shares_rows(p, it);
+                walk.begin(p, it, true);
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    if (st == 1 && shared_rows) break;
+                    if (alive && q_uses[st] > 0) alive = warp_wait(&sh.q_free[st], (uint32_t)(q_uses[st] - 1) & 1u);
+                    if (!alive) break;
+                    ++q_uses[st];
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.q_full[st], (uint32_t)(p.stream_tokens * p.group) * 256u);
+                        for (int blk = 0; blk < 2; ++blk)
+                            tma_load_3d(sQ + st * TILE_BYTES + blk * BLK_BYTES, &tm_q, blk * 64, it.kvh * p.group,
+                                        it.tok0 + st * p.stream_tokens, &sh.q_full[st]);
+                    }
+                }
+                // ---- K
+                for (int t = it.kt0; t < it.kt1 && alive; ++t, ++tiles) {
+                    walk.step_to(p, it, t, true);
+                    if (tiles >= KS) {
+                        const int c = log.back2 >> 1;
+                        alive = warp_wait(&sh.s_full[log.back2 & 1][c % SR], (uint32_t)(c / SR) & 1u);
+                        if (!alive) break;
+                    }
+                    walk.load(&tm_k, p, t, sK + (tiles % KS) * TILE_BYTES, &sh.k_full[tiles % KS]);
+                    log.add(shared_rows, (t - it.kt0) & 1);
+                }
+                if (last) break;
+            }
+            if (alive) {
+                const int slot = items % RING;
+                if (items >= RING) alive = warp_wait(&sh.item_free[slot], (uint32_t)(items / RING - 1) & 1u);
+                if (alive && lane == 0) {
+                    sh.items[slot].kt0 = sh.items[slot].kt1 = 0;
+                    mbar_arrive(&sh.item_full[slot]);
+                }
+            }
+            if (!alive)  // copies in flight land before the block ends
+                for (int t = max(0, tiles - KS); t < tiles; ++t) warp_wait(&sh.k_full[t % KS], (uint32_t)(t / KS) & 1u);
+        } else if (warp == 10) {
+            // ------------------------------------------------ the V ring
+            int tiles = 0;
+            TileLog log;
+            PageWalk walk(p);
+            while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
+                const bool shared_rows = shares_rows(p, it);
+                walk.begin(p, it, false);
+                for (int t = it.kt0; t < it.kt1 && alive; ++t, ++tiles) {
+                    walk.step_to(p, it, t, false);
+                    if (tiles >= VS) {
+                        const int c = log.back1 >> 1;
+                        alive = warp_wait(&sh.o_ready[log.back1 & 1][c & 1], (uint32_t)(c >> 1) & 1u);
+                        if (!alive) break;
+                    }
+                    walk.load(&tm_v, p, t, sV + (tiles % VS) * TILE_BYTES, &sh.v_full[tiles % VS]);
+                    log.add(shared_rows, (t - it.kt0) & 1);
+                }
+                if (!alive) break;
+            }
+            if (!alive)
+                for (int t = max(0, tiles - VS); t < tiles; ++t) warp_wait(&sh.v_full[t % VS], (uint32_t)(t / VS) & 1u);
+        } else if (warp == 9) {
+            // ------------------------------------------------ S = Q K^T, one thread
+            constexpr uint32_t idesc = umma_idesc_f16(BM, BN, 0, 0);
+            constexpr uint32_t hi = umma_desc_hi(1024, UMMA_SW128);
+            const uint32_t q_lo0 = umma_desc_lo(smem_u32(sQ), 16), k_lo0 = umma_desc_lo(smem_u32(sK), 16);
+            int tiles = 0, cnt0 = 0, cnt1 = 0, q_uses[2] = {0, 0};
+            uint32_t made = 0;  // S tiles
+            while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
+                const bool shared_rows = shares_rows(p, it);
+                alive = warp_wait(&sh.q_full[0], (uint32_t)q_uses[0]++ & 1u);
+                if (!shared_rows && alive) alive = warp_wait(&sh.q_full[1], (uint32_t)q_uses[1]++ & 1u);
+                for (int t = it.kt0; t < it.kt1 && alive; ++t, ++tiles) {
+                    alive = warp_wait(&sh.k_full[tiles % KS], (uint32_t)(tiles / KS) & 1u);
+                    const uint32_t k_lo = k_lo0 + (uint32_t)(tiles % KS) * (TILE_BYTES >> 4);
+#pragma unroll 1
+                    for (int st = 0; st < 2 && alive; ++st) {
+                        if (shared_rows && st != ((t - it.kt0) & 1)) continue;
+                        if (made > 0) alive = warp_wait(&sh.s_free, (made - 1) & 1u);
+                        if (!alive) break;
+                        ++made;
+                        tc_fence_after();
+                        if (lane == 0) {
+                            const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
+#pragma unroll
+                            for (int kk = 0; kk < 8; ++kk) {
+                                const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
+                                umma_ss(tbase + COL_S, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc, kk > 0);
+                            }
+                            tc_commit(&sh.s_full[st][(st ? cnt1 : cnt0) % SR]);
+                            // the last S of a stream's rows gives its Q back; shared rows are first merged there
+                            if (t + 1 == it.kt1) tc_commit(shared_rows ? &sh.q_dead : &sh.q_free[st]);
+                        }
+                        __syncwarp();
+                        if (st)
+                            ++cnt1;
+                        else
+                            ++cnt0;
+                    }
+                }
+                if (!alive) break;
+            }
+        } else {
+            // ------------------------------------------------ O += P V, one thread
+            constexpr uint32_t idesc = umma_idesc_f16(BM, D, 0, 1);
+            constexpr uint32_t hi = umma_desc_hi(1024, UMMA_SW128);
+            const uint32_t v_lo0 = umma_desc_lo(smem_u32(sV), BLK_BYTES);
+            int tiles = 0, cnt0 = 0, cnt1 = 0;
+            while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
+                const bool shared_rows = shares_rows(p, it);
+                for (int t = it.kt0; t < it.kt1 && alive; ++t, ++tiles) {
+                    alive = warp_wait(&sh.v_full[tiles % VS], (uint32_t)(tiles / VS) & 1u);
+                    if (!alive) break;
+                    // slots of the last box behind the sequence's last key may hold anything, and 0 * NaN is NaN
+                    const int dead0 = it.kv_total - t * BN, dead1 = min(BN, (dead0 + p.box_rows - 1) / p.box_rows * p.box_rows);
+                    if (dead0 < dead1) {
+                        for (int c = lane; c < (dead1 - dead0) * 16; c += 32)
+                            *reinterpret_cast<uint4*>(sV + (tiles % VS) * TILE_BYTES + ((c >> 3) & 1) * BLK_BYTES +
+                                                      (dead0 + (c >> 4)) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    const uint32_t v_lo = v_lo0 + (uint32_t)(tiles % VS) * (TILE_BYTES >> 4);
+#pragma unroll 1
+                    for (int st = 0; st < 2 && alive; ++st) {
+                        if (shared_rows && st != ((t - it.kt0) & 1)) continue;
+                        const uint32_t p_col = tbase + COL_STREAM + st * STREAM_COLS + COL_P, o_col = tbase + COL_STREAM + st * STREAM_COLS + COL_O;
+                        const bool fresh = shared_rows ? t - it.kt0 < 2 : t == it.kt0;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (alive) alive = warp_wait(&sh.p_full[st][half], (uint32_t)(st ? cnt1 : cnt0) & 1u);
+                            if (!alive) break;
+                            tc_fence_after();
+                            if (lane == 0) {
+#pragma unroll
+                                for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                                    umma_ts(o_col, p_col + kk * 8, umma_desc_pack(v_lo + kk * (2048 >> 4), hi), idesc, kk > 0 || !fresh);
+                                if (half == 1) tc_commit(&sh.o_ready[st][(st ? cnt1 : cnt0) & 1]);
+                            }
+                            __syncwarp();
+                        }
+                        if (st)
+                            ++cnt1;
+                        else
+                            ++cnt0;
+                    }
+                }
+                if (!alive) break;
+            }
+        }
+        if (!alive && lane == 0) atomicOr(p.status, INF_STATUS_WAIT_TIMEOUT);
+    } else {
+        setmaxnreg_inc<224>();
+        // ------------------------------------------------ softmax and epilogue: thread = row
+        const int st = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t col_s = tbase + lanes + COL_S, col_p = tbase + lanes + COL_STREAM + st * STREAM_COLS + COL_P,
+                       col_o = tbase + lanes + COL_STREAM + st * STREAM_COLS + COL_O;
+        const int row_tok = r / p.group, row_head = r - row_tok * p.group;
+        ItemReader reader;
+        Item it;
+        int cnt = 0, pairs = 0, handed = 0, parts_done = 0;  // tiles, items of shared rows, hand-overs, pieces
+        bool ok = true;  // a wait that gave up: the rest runs through without waiting, so that nobody waits for this warp
+        while (reader.next(sh, it) ? it.kt0 < it.kt1 : (ok = false)) {
+            const bool shared_rows = shares_rows(p, it);
+            const int n_all = it.kt1 - it.kt0;
+            const int first_tile = shared_rows ? it.kt0 + st : it.kt0, step = shared_rows ? 2 : 1;
+            const int n = shared_rows ? (n_all + 1 - st) >> 1 : n_all;
+            const int tok_in = shared_rows ? 0 : st * p.stream_tokens;                       // first token of the stream in the item
+            const int rows = min(p.stream_tokens, it.ntok - tok_in) * p.group;               // of the stream
+            const bool valid = r < rows, busy = (warp & 3) * 32 < rows;
+            const int qpos = it.qpos0 + tok_in + row_tok;
+            const int qpos_lo = it.qpos0 + tok_in, qpos_hi = qpos_lo + (rows - 1) / p.group;  // of the stream's rows
+            const int first_key = p.window > 0 ? qpos + 1 - p.window : 0;
+            float m_used = M_INIT, l = 0.f;
+            for (int j = 0; j < n; ++j, ++cnt) {
+                const int k0 = (first_tile + j * step) * BN;
+                if (ok) ok = warp_wait(&sh.s_full[st][cnt % SR], (uint32_t)(cnt / SR) & 1u);
+                tc_fence_after();
+                if (!busy) {  // no row of this warp is used: keep step with the others
+                    if (lane == 0) mbar_arrive(&sh.s_free);
+                    if (j > 0 && ok) ok = warp_wait(&sh.o_ready[st][(cnt - 1) & 1], (uint32_t)((cnt - 1) >> 1) & 1u);
+                    if (lane == 0) {
+                        mbar_arrive(&sh.p_full[st][0]);
+                        mbar_arrive(&sh.p_full[st][1]);
+                    }
+                    continue;
+                }
+                uint32_t x[BN];  // the whole S row of this tile
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) tmem_ld32(col_s + c * 32, x + c * 32);
+                tc_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.s_free);
+                if (k0 + BN - 1 > qpos_lo || (p.window > 0 && k0 < qpos_hi + 1 - p.window)) {
+#pragma unroll
+                    for (int i = 0; i < BN; ++i)
+                        if (k0 + i > qpos || k0 + i < first_key) x[i] = 0xff800000u;  // -inf
+                }
+                float mx[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mx[i] = __uint_as_float(x[i]);
+#pragma unroll
+                for (int i = 8; i < BN; ++i) mx[i & 7] = fmaxf(mx[i & 7], __uint_as_float(x[i]));
+                const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+                const float m_new = fmaxf(m_used, top * p.scale_log2);
+                if (j == 0) {
+                    m_used = m_new;
+                } else {
+                    // P of the tile before is about to be overwritten, and O perhaps scaled: its PV has retired
+                    if (ok) ok = warp_wait(&sh.o_ready[st][(cnt - 1) & 1], (uint32_t)((cnt - 1) >> 1) & 1u);
+                    tc_fence_after();
+                    // A row of O is scaled only when its maximum grew by more than 2^8: until then the weights stay below
+                    // 2^8.  Each row decides for itself, so that its bits do not depend on what else is in the warp.
+                    const bool grew = valid && m_new - m_used > RESCALE_THRESHOLD;
+                    if (__any_sync(0xffffffffu, grew)) {
+                        const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
+                        m_used = grew ? m_new : m_used;
+                        l *= alpha;
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(col_o + c * 32, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st32(col_o + c * 32, o);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                const float neg_m = -m_used;
+                float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) {
+#pragma unroll
+                    for (int i = c * 32; i < c * 32 + 32; i += 2) {
+                        const float p0 = ex2_approx(fmaf(__uint_as_float(x[i]), p.scale_log2, neg_m));
+                        const float p1 = ex2_approx(fmaf(__uint_as_float(x[i + 1]), p.scale_log2, neg_m));
+                        sums[(i >> 1) & 3] += p0 + p1;
+                        x[i / 2] = pack_half2(p0, p1);  // the weights enter PV as fp16: half a step of 2^-11 each
+                    }
+                    tmem_st16(col_p + c * 16, x + c * 16);
+                    if (c & 1) {
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.p_full[st][c >> 1]);
+                    }
+                }
+                l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            }
+            if (n > 0) {
+                if (ok) ok = warp_wait(&sh.o_ready[st][(cnt - 1) & 1], (uint32_t)((cnt - 1) >> 1) & 1u);
+                tc_fence_after();
+            }
+            // ---- shared rows: stream 1 hands its rows over through the Q tiles, which nobody reads any more
+            const bool two = shared_rows && n_all > 1;
+            float* exchange = reinterpret_cast<float*>(sQ) + r * D;  // 16-byte chunks XORed with the row against bank conflicts
+            if (shared_rows && st == 1 && ok) ok = warp_wait(&sh.q_dead, (uint32_t)pairs & 1u);
+            if (two && st == 1) {
+                tc_fence_after();
+                if (busy) {
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(col_o + c * 32, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4*>(exchange + (((c * 8 + i) ^ (r & 31)) << 2)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                    sh.ml[r][0] = m_used;
+                    sh.ml[r][1] = l;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.pair_bar[0]);
+            }
+            const bool writes = st == 0 || !shared_rows;  // this stream's rows leave from here
+            const bool cut = it.pieces > 1;
+            if (writes) {
+                float w0 = 1.f, w1 = 0.f;
+                if (two) {
+                    if (ok) ok = warp_wait(&sh.pair_bar[0], (uint32_t)handed & 1u);
+                    if (busy) {
+                        const float m1 = sh.ml[r][0], l1 = sh.ml[r][1], m_all = fmaxf(m_used, m1);
+                        w0 = ex2_approx(m_used - m_all);
+                        w1 = ex2_approx(m1 - m_all);
+                        l = l * w0 + l1 * w1;
+                        m_used = m_all;
+                    }
+                }
+                if (busy) {
+                    const long long out_row = valid ? (long long)(it.tok0 + tok_in + row_tok) * p.q_heads + it.kvh * p.group + row_head : 0;
+                    const long long part_row = ((long long)(it.ordinal > 0 ? 2 * (it.group + it.ordinal) : 2 * it.group + 1) * 2 + st) * BM + r;
+                    float gain = 1.f;
+                    if (!cut) {
+                        gain = 1.0f / l;
+                        if (p.gate && valid) gain *= softplus(p.gate[out_row]);
+                        w0 *= gain;
+                        w1 *= gain;
+                    } else if (valid) {
+                        p.part_ml[part_row * 2] = m_used;
+                        p.part_ml[part_row * 2 + 1] = l;
+                    }
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(col_o + c * 32, o);
+                        tc_wait_ld();
+                        float y[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * w0;
+                        if (two) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float4 o1 = *reinterpret_cast<const float4*>(exchange + (((c * 8 + i) ^ (r & 31)) << 2));
+                                y[4 * i] = fmaf(o1.x, w1, y[4 * i]);
+                                y[4 * i + 1] = fmaf(o1.y, w1, y[4 * i + 1]);
+                                y[4 * i + 2] = fmaf(o1.z, w1, y[4 * i + 2]);
+                                y[4 * i + 3] = fmaf(o1.w, w1, y[4 * i + 3]);
+                            }
+                        }
+                        if (valid && (cut || !p.out_f16)) {
+                            float4* dst = reinterpret_cast<float4*>(cut ? p.part_acc + part_row * D : (float*)p.out + out_row * D) + c * 8;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                        } else if (valid) {
+                            uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + out_row * D) + c * 4;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                dst[i] = make_uint4(pack_half2(y[8 * i], y[8 * i + 1]), pack_half2(y[8 * i + 2], y[8 * i + 3]),
+                                                    pack_half2(y[8 * i + 4], y[8 * i + 5]), pack_half2(y[8 * i + 6], y[8 * i + 7]));
+                        }
+                        __syncwarp();
+                    }
+                }
+                tc_fence_before();  // the next item's first PV overwrites O
+                if (shared_rows) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.pair_bar[1]);
+                    if (warp == 0) {  // all four warps have read: the Q tile may be filled again
+                        if (ok) ok = warp_wait(&sh.pair_bar[1], (uint32_t)pairs & 1u);
+                        if (lane == 0) mbar_arrive(&sh.q_free[0]);
+                    }
+                }
+            }
+            if (shared_rows) ++pairs;
+            if (two) ++handed;
+            // ---- a cut item: whoever finishes its last piece joins the pieces in the order of the keys
+            if (cut) {
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.part_bar);
+                if (ok) ok = warp_wait(&sh.part_bar, (uint32_t)parts_done & 1u);
+                if (tid == 0) {
+                    const int before = atomicAdd(&p.counters[it.group], 1);
+                    sh.last_piece = before + 1 == it.pieces;
+                    if (before + 1 == it.pieces) p.counters[it.group] = 0;  // for the next launch
+                    mbar_arrive(&sh.flag_bar);
+                }
+                __syncwarp();
+                if (ok) ok = warp_wait(&sh.flag_bar, (uint32_t)parts_done & 1u);
+                ++parts_done;
+                if (sh.last_piece) {
+                    __threadfence();
+                    for (int rr = warp; rr < (shared_rows ? BM : 2 * BM); rr += 8) {  // one warp per row, four values per lane
+                        const int s2 = rr >> 7, r2 = rr & 127, tok2 = s2 * p.stream_tokens + r2 / p.group;
+                        if (r2 >= p.stream_tokens * p.group || tok2 >= it.ntok) continue;
+                        float m = M_INIT;
+                        for (int q = 0; q < it.pieces; ++q) {
+                            const long long row = ((long long)(q > 0 ? 2 * (it.group + q) : 2 * it.group + 1) * 2 + s2) * BM + r2;
+                            m = fmaxf(m, __ldcg(p.part_ml + row * 2));
+                        }
+                        float sum = 0.f;
+                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                        for (int q = 0; q < it.pieces; ++q) {
+                            const long long row = ((long long)(q > 0 ? 2 * (it.group + q) : 2 * it.group + 1) * 2 + s2) * BM + r2;
+                            const float w = ex2_approx(__ldcg(p.part_ml + row * 2) - m);
+                            const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_acc + row * D) + lane);
+                            sum = fmaf(w, __ldcg(p.part_ml + row * 2 + 1), sum);
+                            acc.x = fmaf(w, a.x, acc.x);
+                            acc.y = fmaf(w, a.y, acc.y);
+                            acc.z = fmaf(w, a.z, acc.z);
+                            acc.w = fmaf(w, a.w, acc.w);
+                        }
+                        const long long out_row = (long long)(it.tok0 + tok2) * p.q_heads + it.kvh * p.group + r2 % p.group;
+                        float gain = 1.0f / sum;
+                        if (p.gate) gain *= softplus(p.gate[out_row]);
+                        if (p.out_f16)
+                            reinterpret_cast<uint2*>((__half*)p.out + out_row * D)[lane] =
+                                make_uint2(pack_half2(acc.x * gain, acc.y * gain), pack_half2(acc.z * gain, acc.w * gain));
+                        else
+                            reinterpret_cast<float4*>((float*)p.out + out_row * D)[lane] =
+                                make_float4(acc.x * gain, acc.y * gain, acc.z * gain, acc.w * gain);
+                    }
+                }
+            }
+        }
+        if (!ok && lane == 0) atomicOr(p.status, INF_STATUS_WAIT_TIMEOUT);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) tmem_dealloc(tbase, TMEM_COLS);
+}
+
+// Scratch for the pieces of cut items (a CTA has at most two) and their counters, made by the context's first call.
+int ragged_scratch(inf_ctx* ctx, int grid, float** acc, float** ml, int** counters) {
+    const size_t rows = (size_t)grid * 2 * 2 * BM, bytes = rows * (D + 2) * sizeof(float) + (size_t)grid * sizeof(int);
+    if (!ctx->ragged_scratch) {
+        void* fresh = nullptr;
+        INF_CUDA(ctx, cudaMalloc(&fresh, bytes));
+        const cudaError_t e = cudaMemsetAsync(fresh, 0, bytes, ctx->stream);
+        if (e != cudaSuccess) {
+            cudaFree(fresh);
+            return inf_fail(ctx, INF_E_BACKEND, "gqa_attention_ragged: clearing the scratch failed: %s", cudaGetErrorString(e));
+        }
+        ctx->ragged_scratch = fresh;
+    }
+    *acc = (float*)ctx->ragged_scratch;
+    *ml = *acc + rows * D;
+    *counters = (int*)(*ml + rows * 2);
+    return INF_OK;
 }
 
 }  // namespace
@@ -113,6 +816,8 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
             return inf_fail(ctx, INF_E_CACHE, "%s: page_size must be a positive multiple of 16, got %d", what, pool->page_size);
         if ((long long)pool->num_pages * pool->kv_heads * pool->page_size >= 0x7fffffffLL)
             return inf_fail(ctx, INF_E_CACHE, "%s: the pool's rows must be countable in 31 bits", what);
+        if ((long long)table->max_pages * pool->page_size > (1LL << 30))
+            return inf_fail(ctx, INF_E_CACHE, "%s: a page-table row must not hold more than 2^30 tokens", what);
         if (tokens < 0) return inf_fail(ctx, INF_E_SHAPE, "%s: tokens must not be negative", what);
         if (q_heads <= 0 || q_heads % pool->kv_heads != 0)
             return inf_fail(ctx, INF_E_SHAPE, "%s: q_heads %d must be a positive multiple of kv_heads %d", what, q_heads, pool->kv_heads);
@@ -127,10 +832,8 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
         if (!q_f16 || !q_starts || !out) return inf_fail(ctx, INF_E_ARG, "%s: null pointer", what);
         if (((uintptr_t)q_f16 | (uintptr_t)out | (uintptr_t)pool->k | (uintptr_t)pool->v) & 15u)
             return inf_fail(ctx, INF_E_ARG, "%s: tensors must be 16-byte aligned", what);
+        const int group = q_heads / pool->kv_heads;
         RaggedParams p{};
-        p.q = (const __half*)q_f16;
-        p.k = (const __half*)pool->k;
-        p.v = (const __half*)pool->v;
         p.pages = table->pages;
         p.lens = table->lens;
         p.starts = q_starts;
@@ -139,18 +842,44 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
         p.tokens = tokens;
         p.q_heads = q_heads;
         p.kv_heads = pool->kv_heads;
-        p.group = q_heads / pool->kv_heads;
+        p.group = group;
         p.page_size = pool->page_size;
         p.num_pages = pool->num_pages;
-        p.window = sliding_window;
+        p.window = sliding_window < table->max_pages * pool->page_size ? sliding_window : 0;  // a window no sequence can fill
+        p.stream_tokens = BM / group;
+        p.box_rows = 16;  // the widest box of whole pages' rows: a page holds a multiple of 16
+        while (p.box_rows < BN && pool->page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;
         p.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)D)) * 1.4426950408889634f;
         p.gate = gate;
         p.out = out;
         p.out_f16 = out_dtype == INF_DTYPE_F16;
         p.status = ctx->status;
-        const long long rows = (long long)tokens * q_heads;
-        if ((rows + 7) / 8 > 0x7fffffffLL) return inf_fail(ctx, INF_E_SHAPE, "%s: tokens x heads exceeds the launch grid", what);
-        INF_CUDA(ctx, inf_launch_pdl(ragged_attention_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx->stream, p));
+        const int grid = ctx->sm_count;
+        rc = ragged_scratch(ctx, grid, &p.part_acc, &p.part_ml, &p.counters);
+        if (rc != INF_OK) return rc;
+        CUtensorMap tq, tk, tv;
+        {
+            const uint64_t dims[3] = {D, (uint64_t)q_heads, (uint64_t)tokens}, strides[2] = {D * 2, (uint64_t)q_heads * D * 2};
+            const uint32_t box[3] = {64, (uint32_t)group, (uint32_t)p.stream_tokens};
+            rc = inf_make_tmap(ctx, q_f16, 3, dims, strides, box, &tq);
+            if (rc != INF_OK) return rc;
+        }
+        {
+            const uint64_t dims[2] = {D, (uint64_t)pool->num_pages * pool->kv_heads * pool->page_size}, strides[1] = {D * 2};
+            const uint32_t box[2] = {64, (uint32_t)p.box_rows};
+            rc = inf_make_tmap(ctx, pool->k, 2, dims, strides, box, &tk);
+            if (rc == INF_OK) rc = inf_make_tmap(ctx, pool->v, 2, dims, strides, box, &tv);
+            if (rc != INF_OK) return rc;
+        }
+        constexpr uint32_t attr_bit = 1u << 30;
+        if (!(ctx->func_attr_done & attr_bit)) {
+            INF_CUDA(ctx, cudaFuncSetAttribute(ragged_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+            ctx->func_attr_done |= attr_bit;
+        }
+        {
+            inf_prof_scope prof(ctx, "ragged_attention_kernel");
+            INF_CUDA(ctx, inf_launch_pdl(ragged_attention_kernel, dim3((unsigned)grid), dim3(THREADS), (size_t)SMEM_BYTES, ctx->stream, tq, tk, tv, p));
+        }
         return INF_OK;
     });
 }
