@@ -17,14 +17,20 @@
 // in scratch, and the CTA that finishes its last piece joins them in the order of the keys: nothing depends on timing.
 //
 // Twelve warps:
-//   warps 0-3, 4-7   softmax and epilogue of stream 0 / 1: thread = row = TMEM lane
-//   warp 8           walks the CTA's items, describes each in shared memory for the others, loads Q and the K ring (TMA)
-//   warp 9           issues S = Q K^T (SS, M128 N128 K16) into the ONE S buffer the streams share; a softmax warpgroup
-//                    copies its rows out at once, which frees the buffer for the other stream's next S
+//   warps 0-3, 4-7   softmax and epilogue of stream 0 / 1
+//   warp 8           walks the CTA's items, describes each in shared memory for the others, loads the K ring (TMA)
+//   warp 9           issues every MMA, in the order  S(0) S(1) | PV(0) S(2) | PV(1) S(3) | ...  over the streams' tiles in turn
 //   warp 10          loads the V ring (TMA)
-//   warp 11          issues O += P V (TS: P packed fp16 in TMEM, V MN-major straight from its [key][dim] tile)
-// Rings and counters run on from item to item: the next item's K and V arrive while the last one's rows are written.
-// TMEM: S 128 columns, then per stream P 64 and O 128.  Shared memory: Q 2 x 32 KB, K 3 x 32 KB, V 2 x 32 KB.
+//   warp 11          loads Q
+// S = Q K^T is an SS MMA (M128 N128 K16), O += P V a TS MMA: P, packed fp16, lies over the first half of its own S in TMEM,
+// V is read MN-major straight from its [key][dim] tile.  One thread's MMAs run in order, so S of a stream's next tile, issued
+// behind PV, may overwrite that P, and its barrier also says that PV has retired: a softmax warp waits for one barrier per
+// tile, and while it works on one stream the tensor cores have PV and S of the other.
+// TMEM: S 128 columns and O 128 columns per stream.  Shared memory: Q 2 x 32 KB, K 3 x 32 KB, V 2 x 32 KB.
+//
+// Rows of few items fill few of the 128 lanes, and a warp's exponentials go through one of the four special-function
+// units.  Up to 32 rows (decodes, short drafts) are therefore dealt out to the four lane quarters, and each is held by four
+// threads (16x256 TMEM shape): 32 exponentials a thread and tile instead of 128 on one warp.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -44,9 +50,10 @@ constexpr int SR = 4;                  // rotation of the S barriers: a K slot i
 constexpr int TILE_BYTES = BN * D * 2;  // also the bytes of a stream's Q
 constexpr int BLK_BYTES = BN * 128;    // [128 rows][64 columns] with the 128-byte swizzle
 constexpr int RING = 4;                // item descriptions in flight
+constexpr int FEW_ROWS = 32;           // rows that are dealt out to the lane quarters, eight each
 constexpr float M_INIT = -1.0e30f;
 constexpr float RESCALE_THRESHOLD = 8.0f;
-constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_STREAM = 128, STREAM_COLS = 192, COL_P = 0, COL_O = 64;
+constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;  // 128 columns per stream each
 
 struct Item {
     int b, kvh, tok0, ntok;        // tokens [tok0, tok0 + ntok) of the step
@@ -57,13 +64,12 @@ struct Item {
 
 struct Shared {
     uint64_t q_full[2], q_free[2], k_full[KS], v_full[VS];
-    uint64_t s_full[2][SR];   // S of a stream's tile is in TMEM; its K tile has been read if no other stream reads it
-    uint64_t s_free;          // the S buffer has been copied into registers
+    uint64_t s_full[2][SR];   // S of a stream's tile is in TMEM, PV of its tile before has retired
     uint64_t p_full[2][2];    // keys 0-63 / 64-127 of a stream's P are in TMEM
-    uint64_t o_ready[2][2];   // PV of a stream's tile has retired; its V tile likewise
+    uint64_t o_ready[2][2];   // PV of a stream's tile has retired
     uint64_t item_full[RING], item_free[RING];
-    uint64_t q_dead;          // every S of an item of shared rows has retired: its Q tiles take stream 1's rows
-    uint64_t pair_bar[2], part_bar, flag_bar;  // those rows are there / have been read; pieces
+    uint64_t join[2];         // shared rows: stream 1's maxima and sums are in ml / its O has been read
+    uint64_t part_bar, flag_bar;  // a piece's rows are in scratch / whether it was the last
     uint32_t tmem;
     int last_piece;
     Item items[RING];
@@ -78,6 +84,7 @@ constexpr int SMEM_BYTES = OFF_SHARED + (int)sizeof(Shared);
 static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 
 struct RaggedParams {
+    const __half* q;
     const int *pages, *lens, *starts;
     int batch, max_pages, tokens, q_heads, kv_heads, group, page_size, num_pages, window;
     int stream_tokens;  // Ts
@@ -253,6 +260,218 @@ struct PageWalk {
     }
 };
 
+__device__ __forceinline__ bool few_rows(const RaggedParams& p, const Item& it) { return it.ntok * p.group <= FEW_ROWS; }
+
+// ---- one tile of a stream: S in TMEM -> P over it, and the row's running maximum and sum.  A row of O is scaled only when
+// its maximum grew by more than 2^8: until then the weights stay below 2^8.  Each row decides for itself, so that its bits do
+// not depend on what else is in the warp.  The weights enter PV as fp16, half a step of 2^-11 each; their sum stays in 32 bits.
+
+// thread = row
+__device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, uint32_t col_s, uint32_t col_o, int st, int k0,
+                                             int qpos, int first_key, bool masked, bool valid, bool first, float& m_used, float& l) {
+    const int lane = threadIdx.x & 31;
+    uint32_t x[BN];
+    // the second half of the row arrives while the maximum of the first is taken
+    tmem_ld32(col_s, x);
+    tmem_ld32(col_s + 32, x + 32);
+    tc_wait_ld64(x);
+    tmem_ld32(col_s + 64, x + 64);
+    tmem_ld32(col_s + 96, x + 96);
+    if (masked) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+            if (k0 + i > qpos || k0 + i < first_key) x[i] = 0xff800000u;  // -inf
+    }
+    float mx[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
+#pragma unroll
+    for (int i = 4; i < 60; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[i + e]), __uint_as_float(x[i + 4 + e]));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(x[60 + e]));
+    tc_wait_ld64(x + 64);
+    if (masked) {
+#pragma unroll
+        for (int i = 64; i < BN; ++i)
+            if (k0 + i > qpos || k0 + i < first_key) x[i] = 0xff800000u;
+    }
+#pragma unroll
+    for (int i = 64; i < BN; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[i + e]), __uint_as_float(x[i + 4 + e]));
+    const float m_new = fmaxf(m_used, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2);  // the scale is positive
+    if (first) {
+        m_used = m_new;
+    } else {
+        const bool grew = valid && m_new - m_used > RESCALE_THRESHOLD;
+        if (__any_sync(0xffffffffu, grew)) {
+            const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
+            m_used = grew ? m_new : m_used;
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(col_o + c * 32, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st32(col_o + c * 32, o);
+            }
+            tc_wait_st();
+        }
+    }
+    const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), neg_m2 = pack_f32x2(-m_used, -m_used);
+    uint64_t sums[2] = {0, 0};
+#pragma unroll
+    for (int c = 0; c < BN / 32; ++c) {
+#pragma unroll
+        for (int i = c * 32; i < c * 32 + 32; i += 2) {
+            float a, b;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, neg_m2), a, b);
+            a = ex2_approx(a);
+            b = ex2_approx(b);
+            sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(a, b));
+            x[i / 2] = pack_half2(a, b);
+        }
+        tmem_st16(col_s + c * 16, x + c * 16);
+        if (c & 1) {  // 64 keys of P are there: their PV may start
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.p_full[st][c >> 1]);
+        }
+    }
+    float a, b;
+    unpack_f32x2(add_f32x2(sums[0], sums[1]), a, b);
+    l += a + b;
+}
+
+// a quad of threads = row: thread q of it has columns 8 k + 2 q + {0, 1}; key0 is the first of them
+__device__ __forceinline__ void softmax_tile_few(Shared& sh, const RaggedParams& p, uint32_t col_s, uint32_t col_o, int st, int key0,
+                                                 int qpos, int first_key, bool masked, bool valid, bool first, float& m_used, float& l) {
+    const int lane = threadIdx.x & 31;
+    uint32_t x[64];
+    tmem_ld_16x256(col_s, x);
+    tc_wait_ld64(x);
+    if (masked) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (key0 + 8 * k + e > qpos || key0 + 8 * k + e < first_key) x[4 * k + e] = 0xff800000u;
+    }
+    float mx[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[4]), __uint_as_float(x[5])};
+#pragma unroll
+    for (int k = 2; k < 16; k += 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(x[4 * (k + (e >> 1)) + (e & 1)]));
+    float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float m_new = fmaxf(m_used, top * p.scale_log2);
+    if (first) {
+        m_used = m_new;
+    } else {
+        const bool grew = valid && m_new - m_used > RESCALE_THRESHOLD;
+        if (__any_sync(0xffffffffu, grew)) {
+            const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
+            m_used = grew ? m_new : m_used;
+            l *= alpha;
+            uint32_t o[64];
+            tmem_ld_16x256(col_o, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                o[4 * k] = __float_as_uint(__uint_as_float(o[4 * k]) * alpha);
+                o[4 * k + 1] = __float_as_uint(__uint_as_float(o[4 * k + 1]) * alpha);
+            }
+            tmem_st_16x256(col_o, o);
+            tc_wait_st();
+        }
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint32_t y[16];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float a = ex2_approx(fmaf(__uint_as_float(x[4 * (half * 8 + k)]), p.scale_log2, -m_used));
+            const float b = ex2_approx(fmaf(__uint_as_float(x[4 * (half * 8 + k) + 1]), p.scale_log2, -m_used));
+            sum += a + b;
+            y[2 * k] = pack_half2(a, b);
+            y[2 * k + 1] = 0u;  // lanes 8-15 hold no row
+        }
+        tmem_st_16x128_x8(col_s + half * 32, y);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[st][half]);
+    }
+    l += sum;
+}
+
+// ---- pieces of a cut item: row r of a stream of piece q in the scratch rows
+__device__ __forceinline__ long long piece_row(const Item& it, int q, int st, int r) {
+    return ((long long)(q > 0 ? 2 * (it.group + q) : 2 * it.group + 1) * 2 + st) * BM + r;
+}
+
+// Joins the pieces in the order of the keys.  Each of the eight warps takes every eighth row: first lane = row (maxima, sums,
+// and each piece's weight, left in place of its maximum), then all lanes on one row's 128 values, four rows at a time so that
+// their loads overlap.
+__device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& it, int warp, int lane) {
+    __threadfence();
+    const int per = p.stream_tokens * p.group, all = it.ntok * p.group;  // rows of a full stream, of the item
+    auto scratch_row = [&](int q, int rr) { return rr < per ? piece_row(it, q, 0, rr) : piece_row(it, q, 1, rr - per); };
+    auto out_row = [&](int rr) { return (long long)(it.tok0 + rr / p.group) * p.q_heads + it.kvh * p.group + rr % p.group; };
+    const int mine = warp + 8 * lane;
+    if (mine < all) {
+        float m = M_INIT, sum = 0.f;
+        for (int q = 0; q < it.pieces; ++q) m = fmaxf(m, __ldcg(p.part_ml + scratch_row(q, mine) * 2));
+        for (int q = 0; q < it.pieces; ++q) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + scratch_row(q, mine));
+            sum = fmaf(ex2_approx(ml.x - m), ml.y, sum);
+        }
+        float gain = 1.0f / sum;
+        if (p.gate) gain *= softplus(p.gate[out_row(mine)]);
+        for (int q = 0; q < it.pieces; ++q) {
+            float* at = p.part_ml + scratch_row(q, mine) * 2;
+            __stcg(at, ex2_approx(__ldcg(at) - m) * gain);
+        }
+    }
+    __syncwarp();
+    for (int r0 = warp; r0 < all; r0 += 32) {
+        float4 acc[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int q = 0; q < it.pieces; ++q) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (r0 + 8 * u < all) {
+                    const long long row = scratch_row(q, r0 + 8 * u);
+                    const float w = __ldcg(p.part_ml + row * 2);
+                    const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_acc + row * D) + lane);
+                    acc[u].x = fmaf(w, a.x, acc[u].x);
+                    acc[u].y = fmaf(w, a.y, acc[u].y);
+                    acc[u].z = fmaf(w, a.z, acc[u].z);
+                    acc[u].w = fmaf(w, a.w, acc[u].w);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (r0 + 8 * u < all) {
+                const long long row = out_row(r0 + 8 * u);
+                if (p.out_f16)
+                    reinterpret_cast<uint2*>((__half*)p.out + row * D)[lane] =
+                        make_uint2(pack_half2(acc[u].x, acc[u].y), pack_half2(acc[u].z, acc[u].w));
+                else
+                    reinterpret_cast<float4*>((float*)p.out + row * D)[lane] = acc[u];
+            }
+        }
+    }
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
 ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, RaggedParams p) {
@@ -268,17 +487,14 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             for (int j = 0; j < SR; ++j) mbar_init(&sh.s_full[i][j], 1);
             for (int j = 0; j < 2; ++j) mbar_init(&sh.p_full[i][j], 4);  // one arrival per warp: tcgen05.wait is warp-wide
             for (int j = 0; j < 2; ++j) mbar_init(&sh.o_ready[i][j], 1);
+            mbar_init(&sh.join[i], 4);
         }
         for (int i = 0; i < KS; ++i) mbar_init(&sh.k_full[i], 1);
         for (int i = 0; i < VS; ++i) mbar_init(&sh.v_full[i], 1);
-        mbar_init(&sh.s_free, 4);
         for (int i = 0; i < RING; ++i) {
             mbar_init(&sh.item_full[i], 1);
             mbar_init(&sh.item_free[i], 11);  // every warp but the one that writes
         }
-        mbar_init(&sh.q_dead, 1);
-        mbar_init(&sh.pair_bar[0], 4);
-        mbar_init(&sh.pair_bar[1], 4);
         mbar_init(&sh.part_bar, 8);
         mbar_init(&sh.flag_bar, 1);
         mbar_fence_init();
@@ -309,19 +525,16 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         Item it;
         bool alive = true;
         if (warp == 8) {
-            // ------------------------------------------------ items, Q and the K ring
+            // ------------------------------------------------ items and the K ring
             int b = sh.begin[0], kvh = sh.begin[1], i = sh.begin[2], kt = sh.begin[3], bad = 0;
             const int eb = sh.end[0], ekvh = sh.end[1], ei = sh.end[2], ekt = sh.end[3];
-            bool first = true;     // still in the item the part begins in
-            int items = 0, tiles = 0;
-            TileLog log;
-            int q_uses[2] = {0, 0};
-            int base = -32;
+            bool first = true;  // still in the item the part begins in
+            int items = 0, tiles = 0, base = -32;
             Seq s{0, 0, 0};
+            TileLog log;
             PageWalk walk(p);
-            while (alive) {
+            while (b < p.batch && b <= eb) {
                 // ---- the sequence: metadata of 32 at a time, one per lane
-                if (b >= p.batch || b > eb) break;
                 if (b >= base + 32) {
                     base = b;
                     if (base + lane < p.batch)
@@ -341,17 +554,14 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     continue;
                 }
                 // ---- the item, and how much of it is this CTA's
+                if (b == eb && (kvh > ekvh || (kvh == ekvh && i > ei))) break;
                 const bool last = b == eb && kvh == ekvh && i == ei;
-                const bool past_end = b > eb || (b == eb && (kvh > ekvh || (kvh == ekvh && i > ei)));
-                if (past_end) break;
+                const int* cut = first ? sh.cut[0] : sh.cut[1];
+                it.pieces = first || last ? cut[0] : 1;
+                it.ordinal = first || last ? cut[1] : 0;
+                it.group = first || last ? cut[2] : 0;
                 it.kt0 = first ? kt : h.first_tile(i);
                 it.kt1 = last ? ekt : h.end_tile(i);
-                const int* cut = first ? sh.cut[0] : sh.cut[1];
-                const bool cut_here = first || last;
-                it.pieces = cut_here ? cut[0] : 1;
-                it.ordinal = cut_here ? cut[1] : 0;
-                it.group = cut_here ? cut[2] : 0;
-                first = false;
                 it.b = b;
                 it.kvh = kvh;
                 it.tok0 = start + i * h.T;
@@ -359,45 +569,30 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 it.qpos0 = past + i * h.T;
                 it.kv_total = past + n;
                 it.lowest = h.lo(i);
+                first = false;
                 ++i;
-                if (it.kt0 >= it.kt1) {
-                    if (last) break;
-                    continue;
-                }
-                // ---- tell the others
-                const int slot = items % RING;
-                if (items >= RING) alive = warp_wait(&sh.item_free[slot], (uint32_t)(items / RING - 1) & 1u);
-                if (!alive) break;
-                if (lane == 0) sh.items[slot] = it;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.item_full[slot]);
-                ++items;
-                // ---- Q: a stream's tile is free when its last S has retired (or its rows have been merged)
-                const bool shared_rows = shares_rows(p, it);
-                walk.begin(p, it, true);
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    if (st == 1 && shared_rows) break;
-                    if (alive && q_uses[st] > 0) alive = warp_wait(&sh.q_free[st], (uint32_t)(q_uses[st] - 1) & 1u);
+                if (it.kt0 < it.kt1) {
+                    // ---- tell the others
+                    const int slot = items % RING;
+                    if (items >= RING) alive = warp_wait(&sh.item_free[slot], (uint32_t)(items / RING - 1) & 1u);
                     if (!alive) break;
-                    ++q_uses[st];
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&sh.q_full[st], (uint32_t)(p.stream_tokens * p.group) * 256u);
-                        for (int blk = 0; blk < 2; ++blk)
-                            tma_load_3d(sQ + st * TILE_BYTES + blk * BLK_BYTES, &tm_q, blk * 64, it.kvh * p.group,
-                                        it.tok0 + st * p.stream_tokens, &sh.q_full[st]);
+                    if (lane == 0) sh.items[slot] = it;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.item_full[slot]);
+                    ++items;
+                    const bool shared_rows = shares_rows(p, it);
+                    walk.begin(p, it, true);
+                    for (int t = it.kt0; t < it.kt1; ++t, ++tiles) {
+                        walk.step_to(p, it, t, true);
+                        if (tiles >= KS) {
+                            const int c = log.back2 >> 1;
+                            alive = warp_wait(&sh.s_full[log.back2 & 1][c % SR], (uint32_t)(c / SR) & 1u);
+                            if (!alive) break;
+                        }
+                        walk.load(&tm_k, p, t, sK + (tiles % KS) * TILE_BYTES, &sh.k_full[tiles % KS]);
+                        log.add(shared_rows, (t - it.kt0) & 1);
                     }
-                }
-                // ---- K
-                for (int t = it.kt0; t < it.kt1 && alive; ++t, ++tiles) {
-                    walk.step_to(p, it, t, true);
-                    if (tiles >= KS) {
-                        const int c = log.back2 >> 1;
-                        alive = warp_wait(&sh.s_full[log.back2 & 1][c % SR], (uint32_t)(c / SR) & 1u);
-                        if (!alive) break;
-                    }
-                    walk.load(&tm_k, p, t, sK + (tiles % KS) * TILE_BYTES, &sh.k_full[tiles % KS]);
-                    log.add(shared_rows, (t - it.kt0) & 1);
+                    if (!alive) break;
                 }
                 if (last) break;
             }
@@ -419,7 +614,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
                 const bool shared_rows = shares_rows(p, it);
                 walk.begin(p, it, false);
-                for (int t = it.kt0; t < it.kt1 && alive; ++t, ++tiles) {
+                for (int t = it.kt0; t < it.kt1; ++t, ++tiles) {
                     walk.step_to(p, it, t, false);
                     if (tiles >= VS) {
                         const int c = log.back1 >> 1;
@@ -433,91 +628,131 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             }
             if (!alive)
                 for (int t = max(0, tiles - VS); t < tiles; ++t) warp_wait(&sh.v_full[t % VS], (uint32_t)(t / VS) & 1u);
-        } else if (warp == 9) {
-            // ------------------------------------------------ S = Q K^T, one thread
-            constexpr uint32_t idesc = umma_idesc_f16(BM, BN, 0, 0);
-            constexpr uint32_t hi = umma_desc_hi(1024, UMMA_SW128);
-            const uint32_t q_lo0 = umma_desc_lo(smem_u32(sQ), 16), k_lo0 = umma_desc_lo(smem_u32(sK), 16);
-            int tiles = 0, cnt0 = 0, cnt1 = 0, q_uses[2] = {0, 0};
-            uint32_t made = 0;  // S tiles
+        } else if (warp == 11) {
+            // ------------------------------------------------ Q: a stream's tile is free when its last S has retired
+            int uses0 = 0, uses1 = 0;
             while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
-                const bool shared_rows = shares_rows(p, it);
-                alive = warp_wait(&sh.q_full[0], (uint32_t)q_uses[0]++ & 1u);
-                if (!shared_rows && alive) alive = warp_wait(&sh.q_full[1], (uint32_t)q_uses[1]++ & 1u);
-                for (int t = it.kt0; t < it.kt1 && alive; ++t, ++tiles) {
-                    alive = warp_wait(&sh.k_full[tiles % KS], (uint32_t)(tiles / KS) & 1u);
-                    const uint32_t k_lo = k_lo0 + (uint32_t)(tiles % KS) * (TILE_BYTES >> 4);
-#pragma unroll 1
-                    for (int st = 0; st < 2 && alive; ++st) {
-                        if (shared_rows && st != ((t - it.kt0) & 1)) continue;
-                        if (made > 0) alive = warp_wait(&sh.s_free, (made - 1) & 1u);
-                        if (!alive) break;
-                        ++made;
-                        tc_fence_after();
-                        if (lane == 0) {
-                            const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
-#pragma unroll
-                            for (int kk = 0; kk < 8; ++kk) {
-                                const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
-                                umma_ss(tbase + COL_S, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc, kk > 0);
-                            }
-                            tc_commit(&sh.s_full[st][(st ? cnt1 : cnt0) % SR]);
-                            // the last S of a stream's rows gives its Q back; shared rows are first merged there
-                            if (t + 1 == it.kt1) tc_commit(shared_rows ? &sh.q_dead : &sh.q_free[st]);
-                        }
-                        __syncwarp();
-                        if (st)
-                            ++cnt1;
-                        else
-                            ++cnt0;
-                    }
-                }
+                if (uses0 > 0) alive = warp_wait(&sh.q_free[0], (uint32_t)(uses0 - 1) & 1u);
                 if (!alive) break;
+                ++uses0;
+                if (few_rows(p, it)) {
+                    // row r to lane (r % 4) * 32 + r / 4, with the swizzle that a TMA load would have written
+                    const int chunks = it.ntok * p.group * 16;
+                    for (int c0 = 0; c0 < chunks; c0 += 4 * 32) {
+                        uint4 v[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const int c = c0 + u * 32 + lane, r = c >> 4;
+                            if (c < chunks)
+                                v[u] = *reinterpret_cast<const uint4*>(
+                                    p.q + ((long long)(it.tok0 + r / p.group) * p.q_heads + it.kvh * p.group + r % p.group) * D + (c & 15) * 8);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const int c = c0 + u * 32 + lane, r = c >> 4, row = (r & 3) * 32 + (r >> 2);
+                            if (c < chunks)
+                                *reinterpret_cast<uint4*>(sQ + ((c >> 3) & 1) * BLK_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[u];
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.q_full[0]);
+                    continue;
+                }
+                const uint32_t bytes = (uint32_t)(p.stream_tokens * p.group) * 256u;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sh.q_full[0], bytes);
+                    for (int blk = 0; blk < 2; ++blk)
+                        tma_load_3d(sQ + blk * BLK_BYTES, &tm_q, blk * 64, it.kvh * p.group, it.tok0, &sh.q_full[0]);
+                }
+                if (shares_rows(p, it)) continue;
+                if (uses1 > 0) alive = warp_wait(&sh.q_free[1], (uint32_t)(uses1 - 1) & 1u);
+                if (!alive) break;
+                ++uses1;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sh.q_full[1], bytes);
+                    for (int blk = 0; blk < 2; ++blk)
+                        tma_load_3d(sQ + TILE_BYTES + blk * BLK_BYTES, &tm_q, blk * 64, it.kvh * p.group, it.tok0 + p.stream_tokens,
+                                    &sh.q_full[1]);
+                }
             }
         } else {
-            // ------------------------------------------------ O += P V, one thread
-            constexpr uint32_t idesc = umma_idesc_f16(BM, D, 0, 1);
+            // ------------------------------------------------ every MMA, from one thread
+            constexpr uint32_t idesc_s = umma_idesc_f16(BM, BN, 0, 0), idesc_o = umma_idesc_f16(BM, D, 0, 1);
             constexpr uint32_t hi = umma_desc_hi(1024, UMMA_SW128);
-            const uint32_t v_lo0 = umma_desc_lo(smem_u32(sV), BLK_BYTES);
-            int tiles = 0, cnt0 = 0, cnt1 = 0;
+            const uint32_t q_lo0 = umma_desc_lo(smem_u32(sQ), 16), k_lo0 = umma_desc_lo(smem_u32(sK), 16),
+                           v_lo0 = umma_desc_lo(smem_u32(sV), BLK_BYTES);
+            int k_tiles = 0, v_tiles = 0;                // ring positions: tiles taken so far
+            int made0 = 0, made1 = 0, eaten0 = 0, eaten1 = 0;  // S and PV of each stream
+            int uses0 = 0, uses1 = 0;
             while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
                 const bool shared_rows = shares_rows(p, it);
-                for (int t = it.kt0; t < it.kt1 && alive; ++t, ++tiles) {
-                    alive = warp_wait(&sh.v_full[tiles % VS], (uint32_t)(tiles / VS) & 1u);
-                    if (!alive) break;
-                    // slots of the last box behind the sequence's last key may hold anything, and 0 * NaN is NaN
-                    const int dead0 = it.kv_total - t * BN, dead1 = min(BN, (dead0 + p.box_rows - 1) / p.box_rows * p.box_rows);
-                    if (dead0 < dead1) {
-                        for (int c = lane; c < (dead1 - dead0) * 16; c += 32)
-                            *reinterpret_cast<uint4*>(sV + (tiles % VS) * TILE_BYTES + ((c >> 3) & 1) * BLK_BYTES +
-                                                      (dead0 + (c >> 4)) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        fence_proxy_async_smem();
-                        __syncwarp();
+                const int per = shared_rows ? 1 : 2, steps = (it.kt1 - it.kt0) * per;  // step u: stream u % 2, tile u / per
+                alive = warp_wait(&sh.q_full[0], (uint32_t)uses0++ & 1u);
+                auto scores = [&](int u) {  // S of step u
+                    const int st = u & 1;
+                    if (!shared_rows && u == 1 && alive) alive = warp_wait(&sh.q_full[1], (uint32_t)uses1++ & 1u);
+                    if (shared_rows || st == 0) {
+                        if (alive) alive = warp_wait(&sh.k_full[k_tiles % KS], (uint32_t)(k_tiles / KS) & 1u);
+                        ++k_tiles;
                     }
-                    const uint32_t v_lo = v_lo0 + (uint32_t)(tiles % VS) * (TILE_BYTES >> 4);
+                    if (!alive) return;
+                    if (lane == 0) {
+                        const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
+                        const uint32_t k_lo = k_lo0 + (uint32_t)((k_tiles - 1) % KS) * (TILE_BYTES >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
+                            umma_ss(tbase + COL_S + st * BN, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
+                        }
+                        tc_commit(&sh.s_full[st][(st ? made1 : made0) % SR]);
+                        if (u + (shared_rows ? 1 : 2) >= steps) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
+                    }
+                    __syncwarp();
+                    if (st)
+                        ++made1;
+                    else
+                        ++made0;
+                };
+                scores(0);
+                if (steps > 1) scores(1);
 #pragma unroll 1
-                    for (int st = 0; st < 2 && alive; ++st) {
-                        if (shared_rows && st != ((t - it.kt0) & 1)) continue;
-                        const uint32_t p_col = tbase + COL_STREAM + st * STREAM_COLS + COL_P, o_col = tbase + COL_STREAM + st * STREAM_COLS + COL_O;
-                        const bool fresh = shared_rows ? t - it.kt0 < 2 : t == it.kt0;
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            if (alive) alive = warp_wait(&sh.p_full[st][half], (uint32_t)(st ? cnt1 : cnt0) & 1u);
-                            if (!alive) break;
-                            tc_fence_after();
-                            if (lane == 0) {
-#pragma unroll
-                                for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                                    umma_ts(o_col, p_col + kk * 8, umma_desc_pack(v_lo + kk * (2048 >> 4), hi), idesc, kk > 0 || !fresh);
-                                if (half == 1) tc_commit(&sh.o_ready[st][(st ? cnt1 : cnt0) & 1]);
-                            }
+                for (int u = 0; u < steps && alive; ++u) {
+                    const int st = u & 1, t = it.kt0 + (shared_rows ? u : u >> 1);
+                    if (shared_rows || st == 0) {
+                        alive = warp_wait(&sh.v_full[v_tiles % VS], (uint32_t)(v_tiles / VS) & 1u);
+                        ++v_tiles;
+                        if (!alive) break;
+                        // slots of the last box behind the sequence's last key may hold anything, and 0 * NaN is NaN
+                        const int dead0 = it.kv_total - t * BN, dead1 = min(BN, (dead0 + p.box_rows - 1) / p.box_rows * p.box_rows);
+                        if (dead0 < dead1) {
+                            for (int c = lane; c < (dead1 - dead0) * 16; c += 32)
+                                *reinterpret_cast<uint4*>(sV + ((v_tiles - 1) % VS) * TILE_BYTES + ((c >> 3) & 1) * BLK_BYTES +
+                                                          (dead0 + (c >> 4)) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            fence_proxy_async_smem();
                             __syncwarp();
                         }
-                        if (st)
-                            ++cnt1;
-                        else
-                            ++cnt0;
                     }
+                    const uint32_t v_lo = v_lo0 + (uint32_t)((v_tiles - 1) % VS) * (TILE_BYTES >> 4);
+                    const uint32_t p_col = tbase + COL_S + st * BN, o_col = tbase + COL_O + st * D;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {  // the halves of P arrive separately
+                        if (alive) alive = warp_wait(&sh.p_full[st][half], (uint32_t)(st ? eaten1 : eaten0) & 1u);
+                        if (!alive) break;
+                        tc_fence_after();
+                        if (lane == 0) {
+#pragma unroll
+                            for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                                umma_ts(o_col, p_col + kk * 8, umma_desc_pack(v_lo + kk * (2048 >> 4), hi), idesc_o, kk > 0 || u > 1);
+                            if (half == 1) tc_commit(&sh.o_ready[st][(st ? eaten1 : eaten0) & 1]);
+                        }
+                        __syncwarp();
+                    }
+                    if (st)
+                        ++eaten1;
+                    else
+                        ++eaten0;
+                    if (alive && u + 2 < steps) scores(u + 2);
                 }
                 if (!alive) break;
             }
@@ -525,204 +760,150 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         if (!alive && lane == 0) atomicOr(p.status, INF_STATUS_WAIT_TIMEOUT);
     } else {
         setmaxnreg_inc<224>();
-        // ------------------------------------------------ softmax and epilogue: thread = row
-        const int st = warp >> 2, r = tid & 127;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t col_s = tbase + lanes + COL_S, col_p = tbase + lanes + COL_STREAM + st * STREAM_COLS + COL_P,
-                       col_o = tbase + lanes + COL_STREAM + st * STREAM_COLS + COL_O;
-        const int row_tok = r / p.group, row_head = r - row_tok * p.group;
+        // ------------------------------------------------ softmax and epilogue
+        const int st = warp >> 2, quarter = warp & 3;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t col_s = tbase + lanes + COL_S + st * BN, col_o = tbase + lanes + COL_O + st * D;
         ItemReader reader;
         Item it;
-        int cnt = 0, pairs = 0, handed = 0, parts_done = 0;  // tiles, items of shared rows, hand-overs, pieces
+        int cnt = 0, joins = 0, parts_done = 0;  // tiles, items that both streams' rows were joined in, pieces
         bool ok = true;  // a wait that gave up: the rest runs through without waiting, so that nobody waits for this warp
         while (reader.next(sh, it) ? it.kt0 < it.kt1 : (ok = false)) {
-            const bool shared_rows = shares_rows(p, it);
+            const bool shared_rows = shares_rows(p, it), few = few_rows(p, it);
             const int n_all = it.kt1 - it.kt0;
             const int first_tile = shared_rows ? it.kt0 + st : it.kt0, step = shared_rows ? 2 : 1;
             const int n = shared_rows ? (n_all + 1 - st) >> 1 : n_all;
-            const int tok_in = shared_rows ? 0 : st * p.stream_tokens;                       // first token of the stream in the item
-            const int rows = min(p.stream_tokens, it.ntok - tok_in) * p.group;               // of the stream
-            const bool valid = r < rows, busy = (warp & 3) * 32 < rows;
-            const int qpos = it.qpos0 + tok_in + row_tok;
+            const int tok_in = shared_rows ? 0 : st * p.stream_tokens;          // first token of the stream in the item
+            const int rows = min(p.stream_tokens, it.ntok - tok_in) * p.group;  // of the stream
+            // this thread's row: its lane's, or with few rows the one it shares with the three other threads of its quad
+            const int r = few ? (lane >> 2) * 4 + quarter : quarter * 32 + lane;
+            const bool valid = r < rows, busy = few ? quarter < rows : quarter * 32 < rows;
+            const int row_tok = r / p.group;
             const int qpos_lo = it.qpos0 + tok_in, qpos_hi = qpos_lo + (rows - 1) / p.group;  // of the stream's rows
-            const int first_key = p.window > 0 ? qpos + 1 - p.window : 0;
+            const int qpos = qpos_lo + row_tok, first_key = p.window > 0 ? qpos + 1 - p.window : 0;
             float m_used = M_INIT, l = 0.f;
             for (int j = 0; j < n; ++j, ++cnt) {
                 const int k0 = (first_tile + j * step) * BN;
                 if (ok) ok = warp_wait(&sh.s_full[st][cnt % SR], (uint32_t)(cnt / SR) & 1u);
                 tc_fence_after();
+                const bool masked = k0 + BN - 1 > qpos_lo || (p.window > 0 && k0 < qpos_hi + 1 - p.window);
                 if (!busy) {  // no row of this warp is used: keep step with the others
-                    if (lane == 0) mbar_arrive(&sh.s_free);
-                    if (j > 0 && ok) ok = warp_wait(&sh.o_ready[st][(cnt - 1) & 1], (uint32_t)((cnt - 1) >> 1) & 1u);
-                    if (lane == 0) {
-                        mbar_arrive(&sh.p_full[st][0]);
-                        mbar_arrive(&sh.p_full[st][1]);
-                    }
-                    continue;
-                }
-                uint32_t x[BN];  // the whole S row of this tile
-#pragma unroll
-                for (int c = 0; c < BN / 32; ++c) tmem_ld32(col_s + c * 32, x + c * 32);
-                tc_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.s_free);
-                if (k0 + BN - 1 > qpos_lo || (p.window > 0 && k0 < qpos_hi + 1 - p.window)) {
-#pragma unroll
-                    for (int i = 0; i < BN; ++i)
-                        if (k0 + i > qpos || k0 + i < first_key) x[i] = 0xff800000u;  // -inf
-                }
-                float mx[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) mx[i] = __uint_as_float(x[i]);
-#pragma unroll
-                for (int i = 8; i < BN; ++i) mx[i & 7] = fmaxf(mx[i & 7], __uint_as_float(x[i]));
-                const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-                const float m_new = fmaxf(m_used, top * p.scale_log2);
-                if (j == 0) {
-                    m_used = m_new;
+                    if (lane < 2) mbar_arrive(&sh.p_full[st][lane]);
+                } else if (few) {
+                    softmax_tile_few(sh, p, col_s, col_o, st, k0 + 2 * (lane & 3), qpos, first_key, masked, valid, j == 0, m_used, l);
                 } else {
-                    // P of the tile before is about to be overwritten, and O perhaps scaled: its PV has retired
-                    if (ok) ok = warp_wait(&sh.o_ready[st][(cnt - 1) & 1], (uint32_t)((cnt - 1) >> 1) & 1u);
-                    tc_fence_after();
-                    // A row of O is scaled only when its maximum grew by more than 2^8: until then the weights stay below
-                    // 2^8.  Each row decides for itself, so that its bits do not depend on what else is in the warp.
-                    const bool grew = valid && m_new - m_used > RESCALE_THRESHOLD;
-                    if (__any_sync(0xffffffffu, grew)) {
-                        const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
-                        m_used = grew ? m_new : m_used;
-                        l *= alpha;
-#pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(col_o + c * 32, o);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st32(col_o + c * 32, o);
-                        }
-                        tc_wait_st();
-                    }
+                    softmax_tile(sh, p, col_s, col_o, st, k0, qpos, first_key, masked, valid, j == 0, m_used, l);
                 }
-                const float neg_m = -m_used;
-                float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < BN / 32; ++c) {
-#pragma unroll
-                    for (int i = c * 32; i < c * 32 + 32; i += 2) {
-                        const float p0 = ex2_approx(fmaf(__uint_as_float(x[i]), p.scale_log2, neg_m));
-                        const float p1 = ex2_approx(fmaf(__uint_as_float(x[i + 1]), p.scale_log2, neg_m));
-                        sums[(i >> 1) & 3] += p0 + p1;
-                        x[i / 2] = pack_half2(p0, p1);  // the weights enter PV as fp16: half a step of 2^-11 each
-                    }
-                    tmem_st16(col_p + c * 16, x + c * 16);
-                    if (c & 1) {
-                        tc_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.p_full[st][c >> 1]);
-                    }
-                }
-                l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
             }
             if (n > 0) {
                 if (ok) ok = warp_wait(&sh.o_ready[st][(cnt - 1) & 1], (uint32_t)((cnt - 1) >> 1) & 1u);
                 tc_fence_after();
             }
-            // ---- shared rows: stream 1 hands its rows over through the Q tiles, which nobody reads any more
-            const bool two = shared_rows && n_all > 1;
-            float* exchange = reinterpret_cast<float*>(sQ) + r * D;  // 16-byte chunks XORed with the row against bank conflicts
-            if (shared_rows && st == 1 && ok) ok = warp_wait(&sh.q_dead, (uint32_t)pairs & 1u);
-            if (two && st == 1) {
-                tc_fence_after();
-                if (busy) {
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(col_o + c * 32, o);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<uint4*>(exchange + (((c * 8 + i) ^ (r & 31)) << 2)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    }
-                    sh.ml[r][0] = m_used;
-                    sh.ml[r][1] = l;
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.pair_bar[0]);
+            if (few) {  // each thread of the quad has summed its own columns
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
             }
-            const bool writes = st == 0 || !shared_rows;  // this stream's rows leave from here
+            // ---- shared rows: stream 0 joins the two; the same lanes hold the same rows, so it reads stream 1's O in place
+            const bool two = shared_rows && n_all > 1;
             const bool cut = it.pieces > 1;
-            if (writes) {
+            if (two && st == 1) {
+                sh.ml[quarter * 32 + lane][0] = m_used;
+                sh.ml[quarter * 32 + lane][1] = l;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.join[0]);
+                if (ok) ok = warp_wait(&sh.join[1], (uint32_t)joins & 1u);  // before this stream's next PV
+            }
+            if (st == 0 || !shared_rows) {
                 float w0 = 1.f, w1 = 0.f;
                 if (two) {
-                    if (ok) ok = warp_wait(&sh.pair_bar[0], (uint32_t)handed & 1u);
-                    if (busy) {
-                        const float m1 = sh.ml[r][0], l1 = sh.ml[r][1], m_all = fmaxf(m_used, m1);
-                        w0 = ex2_approx(m_used - m_all);
-                        w1 = ex2_approx(m1 - m_all);
-                        l = l * w0 + l1 * w1;
-                        m_used = m_all;
-                    }
+                    if (ok) ok = warp_wait(&sh.join[0], (uint32_t)joins & 1u);
+                    tc_fence_after();
+                    const float m1 = sh.ml[quarter * 32 + lane][0], m_all = fmaxf(m_used, m1);
+                    w0 = ex2_approx(m_used - m_all);
+                    w1 = ex2_approx(m1 - m_all);
+                    l = l * w0 + sh.ml[quarter * 32 + lane][1] * w1;
+                    m_used = m_all;
                 }
                 if (busy) {
-                    const long long out_row = valid ? (long long)(it.tok0 + tok_in + row_tok) * p.q_heads + it.kvh * p.group + row_head : 0;
-                    const long long part_row = ((long long)(it.ordinal > 0 ? 2 * (it.group + it.ordinal) : 2 * it.group + 1) * 2 + st) * BM + r;
-                    float gain = 1.f;
+                    const long long out_row =
+                        valid ? (long long)(it.tok0 + tok_in + row_tok) * p.q_heads + it.kvh * p.group + (r - row_tok * p.group) : 0;
+                    const long long part_row = piece_row(it, it.ordinal, st, r);
                     if (!cut) {
-                        gain = 1.0f / l;
+                        float gain = 1.0f / l;
                         if (p.gate && valid) gain *= softplus(p.gate[out_row]);
                         w0 *= gain;
                         w1 *= gain;
-                    } else if (valid) {
+                    } else if (valid && (!few || (lane & 3) == 0)) {
                         p.part_ml[part_row * 2] = m_used;
                         p.part_ml[part_row * 2 + 1] = l;
                     }
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(col_o + c * 32, o);
-                        tc_wait_ld();
+                    float* out32 = cut ? p.part_acc + part_row * D : (float*)p.out + out_row * D;  // f32 rows
+                    __half* out16 = cut || !p.out_f16 ? nullptr : (__half*)p.out + out_row * D;
+                    if (few) {
+                        uint32_t o[64];
                         float y[32];
+                        tmem_ld_16x256(col_o, o);
+                        tc_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * w0;
+                        for (int k = 0; k < 16; ++k) {
+                            y[2 * k] = __uint_as_float(o[4 * k]) * w0;
+                            y[2 * k + 1] = __uint_as_float(o[4 * k + 1]) * w0;
+                        }
                         if (two) {
+                            tmem_ld_16x256(col_o + D, o);
+                            tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float4 o1 = *reinterpret_cast<const float4*>(exchange + (((c * 8 + i) ^ (r & 31)) << 2));
-                                y[4 * i] = fmaf(o1.x, w1, y[4 * i]);
-                                y[4 * i + 1] = fmaf(o1.y, w1, y[4 * i + 1]);
-                                y[4 * i + 2] = fmaf(o1.z, w1, y[4 * i + 2]);
-                                y[4 * i + 3] = fmaf(o1.w, w1, y[4 * i + 3]);
+                            for (int k = 0; k < 16; ++k) {
+                                y[2 * k] = fmaf(__uint_as_float(o[4 * k]), w1, y[2 * k]);
+                                y[2 * k + 1] = fmaf(__uint_as_float(o[4 * k + 1]), w1, y[2 * k + 1]);
                             }
                         }
-                        if (valid && (cut || !p.out_f16)) {
-                            float4* dst = reinterpret_cast<float4*>(cut ? p.part_acc + part_row * D : (float*)p.out + out_row * D) + c * 8;
+                        if (valid) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                        } else if (valid) {
-                            uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + out_row * D) + c * 4;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                dst[i] = make_uint4(pack_half2(y[8 * i], y[8 * i + 1]), pack_half2(y[8 * i + 2], y[8 * i + 3]),
-                                                    pack_half2(y[8 * i + 4], y[8 * i + 5]), pack_half2(y[8 * i + 6], y[8 * i + 7]));
+                            for (int k = 0; k < 16; ++k) {
+                                const int d = 8 * k + 2 * (lane & 3);
+                                if (out16)
+                                    *reinterpret_cast<uint32_t*>(out16 + d) = pack_half2(y[2 * k], y[2 * k + 1]);
+                                else
+                                    *reinterpret_cast<float2*>(out32 + d) = make_float2(y[2 * k], y[2 * k + 1]);
+                            }
                         }
-                        __syncwarp();
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            float y[32];
+                            tmem_ld32(col_o + c * 32, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * w0;
+                            if (two) {
+                                tmem_ld32(col_o + D + c * 32, o);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) y[i] = fmaf(__uint_as_float(o[i]), w1, y[i]);
+                            }
+                            if (valid && out16) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 8)
+                                    *reinterpret_cast<uint4*>(out16 + c * 32 + i) =
+                                        make_uint4(pack_half2(y[i], y[i + 1]), pack_half2(y[i + 2], y[i + 3]), pack_half2(y[i + 4], y[i + 5]),
+                                                   pack_half2(y[i + 6], y[i + 7]));
+                            } else if (valid) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4)
+                                    *reinterpret_cast<float4*>(out32 + c * 32 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                            }
+                            __syncwarp();
+                        }
                     }
                 }
                 tc_fence_before();  // the next item's first PV overwrites O
-                if (shared_rows) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.pair_bar[1]);
-                    if (warp == 0) {  // all four warps have read: the Q tile may be filled again
-                        if (ok) ok = warp_wait(&sh.pair_bar[1], (uint32_t)pairs & 1u);
-                        if (lane == 0) mbar_arrive(&sh.q_free[0]);
-                    }
-                }
+                __syncwarp();
+                if (two && lane == 0) mbar_arrive(&sh.join[1]);
             }
-            if (shared_rows) ++pairs;
-            if (two) ++handed;
+            if (two) ++joins;
             // ---- a cut item: whoever finishes its last piece joins the pieces in the order of the keys
             if (cut) {
                 __threadfence();
@@ -738,40 +919,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 __syncwarp();
                 if (ok) ok = warp_wait(&sh.flag_bar, (uint32_t)parts_done & 1u);
                 ++parts_done;
-                if (sh.last_piece) {
-                    __threadfence();
-                    for (int rr = warp; rr < (shared_rows ? BM : 2 * BM); rr += 8) {  // one warp per row, four values per lane
-                        const int s2 = rr >> 7, r2 = rr & 127, tok2 = s2 * p.stream_tokens + r2 / p.group;
-                        if (r2 >= p.stream_tokens * p.group || tok2 >= it.ntok) continue;
-                        float m = M_INIT;
-                        for (int q = 0; q < it.pieces; ++q) {
-                            const long long row = ((long long)(q > 0 ? 2 * (it.group + q) : 2 * it.group + 1) * 2 + s2) * BM + r2;
-                            m = fmaxf(m, __ldcg(p.part_ml + row * 2));
-                        }
-                        float sum = 0.f;
-                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                        for (int q = 0; q < it.pieces; ++q) {
-                            const long long row = ((long long)(q > 0 ? 2 * (it.group + q) : 2 * it.group + 1) * 2 + s2) * BM + r2;
-                            const float w = ex2_approx(__ldcg(p.part_ml + row * 2) - m);
-                            const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_acc + row * D) + lane);
-                            sum = fmaf(w, __ldcg(p.part_ml + row * 2 + 1), sum);
-                            acc.x = fmaf(w, a.x, acc.x);
-                            acc.y = fmaf(w, a.y, acc.y);
-                            acc.z = fmaf(w, a.z, acc.z);
-                            acc.w = fmaf(w, a.w, acc.w);
-                        }
-                        const long long out_row = (long long)(it.tok0 + tok2) * p.q_heads + it.kvh * p.group + r2 % p.group;
-                        float gain = 1.0f / sum;
-                        if (p.gate) gain *= softplus(p.gate[out_row]);
-                        if (p.out_f16)
-                            reinterpret_cast<uint2*>((__half*)p.out + out_row * D)[lane] =
-                                make_uint2(pack_half2(acc.x * gain, acc.y * gain), pack_half2(acc.z * gain, acc.w * gain));
-                        else
-                            reinterpret_cast<float4*>((float*)p.out + out_row * D)[lane] =
-                                make_float4(acc.x * gain, acc.y * gain, acc.z * gain, acc.w * gain);
-                    }
-                }
+                if (sh.last_piece) join_pieces(p, it, warp, lane);
             }
         }
         if (!ok && lane == 0) atomicOr(p.status, INF_STATUS_WAIT_TIMEOUT);
@@ -834,6 +982,7 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
             return inf_fail(ctx, INF_E_ARG, "%s: tensors must be 16-byte aligned", what);
         const int group = q_heads / pool->kv_heads;
         RaggedParams p{};
+        p.q = (const __half*)q_f16;
         p.pages = table->pages;
         p.lens = table->lens;
         p.starts = q_starts;

@@ -13,6 +13,7 @@ constexpr int RAGGED_TILE = 128;  // keys of a tile
 // tiles or more also keep two cuts of one item from falling on the same tile.
 constexpr int RAGGED_ITEM_COST = 128;
 constexpr int RAGGED_MIN_PART = 3 * RAGGED_TILE;
+constexpr int RAGGED_SNAP = 2;
 
 // The items of T tokens of one KV head of a sequence: n new tokens behind `past` cached ones.
 struct RaggedHead {
@@ -44,11 +45,14 @@ struct RaggedHead {
         }
         return a;
     }
-    // the key tile at which a cut z into the cost of item i falls: one of its ends where it is near them
+    // The key tile at which a cut z into the cost of item i falls.  A cut within RAGGED_SNAP tiles of an end of an item of two
+    // streams goes there: the pieces of up to 256 rows cost more than so many tiles.
     RAGGED_FN int tile_at(int i, long long z) const {
+        const int snap = n - i * T > T / 2 ? RAGGED_SNAP : 0;
         if (z <= RAGGED_ITEM_COST) return first_tile(i);
-        const int key = lo(i) + (int)(z - RAGGED_ITEM_COST);
-        return (int)most(first_tile(i), least(end_tile(i), (key + RAGGED_TILE / 2) / RAGGED_TILE));
+        const int tile = (lo(i) + (int)(z - RAGGED_ITEM_COST) + RAGGED_TILE / 2) / RAGGED_TILE;
+        if (tile <= first_tile(i) + snap) return first_tile(i);
+        return tile >= end_tile(i) - snap ? end_tile(i) : tile;
     }
 };
 
