@@ -266,47 +266,56 @@ __device__ __forceinline__ bool few_rows(const RaggedParams& p, const Item& it) 
 // its maximum grew by more than 2^8: until then the weights stay below 2^8.  Each row decides for itself, so that its bits do
 // not depend on what else is in the warp.  The weights enter PV as fp16, half a step of 2^-11 each; their sum stays in 32 bits.
 
-// thread = row
-__device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, uint32_t col_s, uint32_t col_o, int st, int k0,
-                                             int qpos, int first_key, bool masked, bool valid, bool first, float& m_used, float& l) {
-    const int lane = threadIdx.x & 31;
-    uint32_t x[BN];
-    // the second half of the row arrives while the maximum of the first is taken
-    tmem_ld32(col_s, x);
-    tmem_ld32(col_s + 32, x + 32);
-    tc_wait_ld64(x);
-    tmem_ld32(col_s + 64, x + 64);
-    tmem_ld32(col_s + 96, x + 96);
-    if (masked) {
+// weights of 64 keys of a row, packed, and their sum
+__device__ __forceinline__ void exponentials(const uint32_t* x, float scale_log2, float m, uint32_t* packed, uint64_t* sums) {
+    const uint64_t scale2 = pack_f32x2(scale_log2, scale_log2), neg_m2 = pack_f32x2(-m, -m);
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-            if (k0 + i > qpos || k0 + i < first_key) x[i] = 0xff800000u;  // -inf
+    for (int i = 0; i < 64; i += 2) {
+        float a, b;
+        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, neg_m2), a, b);
+        a = ex2_approx(a);
+        b = ex2_approx(b);
+        sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(a, b));
+        packed[i / 2] = pack_half2(a, b);
     }
+}
+__device__ __forceinline__ void mask_keys(uint32_t* x, int k0, int qpos, int first_key) {
+#pragma unroll
+    for (int i = 0; i < 64; ++i)
+        if (k0 + i > qpos || k0 + i < first_key) x[i] = 0xff800000u;  // -inf
+}
+__device__ __forceinline__ float max_of(const uint32_t* x) {
     float mx[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
 #pragma unroll
     for (int i = 4; i < 60; i += 8)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[i + e]), __uint_as_float(x[i + 4 + e]));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(x[60 + e]));
+    return max3(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), fmaxf(__uint_as_float(x[60]), __uint_as_float(x[61])),
+                fmaxf(__uint_as_float(x[62]), __uint_as_float(x[63])));
+}
+
+// thread = row.  The weights of the first 64 keys are taken with the maximum so far while the rest of the row arrives and
+// its maximum is found; they are taken again (from S, which P has not covered yet) where that one turns out 2^8 larger.
+__device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, uint32_t col_s, uint32_t col_o, int st, int k0,
+                                             int qpos, int first_key, bool masked, bool valid, bool first, float& m_used, float& l) {
+    const int lane = threadIdx.x & 31;
+    uint32_t x[BN], packed[32];
+    uint64_t sums[2] = {0, 0};
+    tmem_ld32(col_s, x);
+    tmem_ld32(col_s + 32, x + 32);
+    tc_wait_ld64(x);
+    tmem_ld32(col_s + 64, x + 64);
+    tmem_ld32(col_s + 96, x + 96);
+    if (masked) mask_keys(x, k0, qpos, first_key);
+    const float top0 = max_of(x);
+    if (!first) exponentials(x, p.scale_log2, m_used, packed, sums);
     tc_wait_ld64(x + 64);
-    if (masked) {
-#pragma unroll
-        for (int i = 64; i < BN; ++i)
-            if (k0 + i > qpos || k0 + i < first_key) x[i] = 0xff800000u;
-    }
-#pragma unroll
-    for (int i = 64; i < BN; i += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[i + e]), __uint_as_float(x[i + 4 + e]));
-    const float m_new = fmaxf(m_used, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2);  // the scale is positive
-    if (first) {
-        m_used = m_new;
-    } else {
-        const bool grew = valid && m_new - m_used > RESCALE_THRESHOLD;
-        if (__any_sync(0xffffffffu, grew)) {
+    if (masked) mask_keys(x + 64, k0 + 64, qpos, first_key);
+    const float m_new = fmaxf(m_used, fmaxf(top0, max_of(x + 64)) * p.scale_log2);  // the scale is positive
+    const bool grew = first || (valid && m_new - m_used > RESCALE_THRESHOLD);
+    if (__any_sync(0xffffffffu, grew)) {
+        if (!first) {
             const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
-            m_used = grew ? m_new : m_used;
             l *= alpha;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
@@ -318,29 +327,26 @@ __device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, 
                 tmem_st32(col_o + c * 32, o);
             }
             tc_wait_st();
+            tmem_ld32(col_s, x);
+            tmem_ld32(col_s + 32, x + 32);
+            tc_wait_ld64(x);
+            if (masked) mask_keys(x, k0, qpos, first_key);
         }
+        m_used = grew ? m_new : m_used;
+        sums[0] = sums[1] = 0;
+        exponentials(x, p.scale_log2, m_used, packed, sums);
     }
-    const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), neg_m2 = pack_f32x2(-m_used, -m_used);
-    uint64_t sums[2] = {0, 0};
-#pragma unroll
-    for (int c = 0; c < BN / 32; ++c) {
-#pragma unroll
-        for (int i = c * 32; i < c * 32 + 32; i += 2) {
-            float a, b;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, neg_m2), a, b);
-            a = ex2_approx(a);
-            b = ex2_approx(b);
-            sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(a, b));
-            x[i / 2] = pack_half2(a, b);
-        }
-        tmem_st16(col_s + c * 16, x + c * 16);
-        if (c & 1) {  // 64 keys of P are there: their PV may start
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.p_full[st][c >> 1]);
-        }
-    }
+    tmem_st32(col_s, packed);
+    tc_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.p_full[st][0]);  // 64 keys of P are there: their PV may start
+    exponentials(x + 64, p.scale_log2, m_used, packed, sums);
+    tmem_st32(col_s + 32, packed);
+    tc_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.p_full[st][1]);
     float a, b;
     unpack_f32x2(add_f32x2(sums[0], sums[1]), a, b);
     l += a + b;
@@ -520,7 +526,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     if (!has_work) {
         // nothing to do for this CTA
     } else if (warp >= 8) {
-        setmaxnreg_dec<56>();
+        setmaxnreg_dec<72>();
         ItemReader reader;
         Item it;
         bool alive = true;
@@ -759,7 +765,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         }
         if (!alive && lane == 0) atomicOr(p.status, INF_STATUS_WAIT_TIMEOUT);
     } else {
-        setmaxnreg_inc<224>();
+        setmaxnreg_inc<216>();
         // ------------------------------------------------ softmax and epilogue
         const int st = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
