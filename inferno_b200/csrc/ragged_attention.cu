@@ -68,6 +68,7 @@ struct Shared {
     uint64_t p_full[2][2];    // keys 0-63 / 64-127 of a stream's P are in TMEM
     uint64_t o_ready[2][2];   // PV of a stream's tile has retired
     uint64_t item_full[RING], item_free[RING];
+    uint64_t v_patched[VS];   // dead slots of the V tile in this ring slot have been cleared
     uint64_t join[2];         // shared rows: stream 1's maxima and sums are in ml / its O has been read
     uint64_t part_bar, flag_bar;  // a piece's rows are in scratch / whether it was the last
     uint32_t tmem;
@@ -199,10 +200,24 @@ struct ItemReader {
         ++count;
         return true;
     }
+    __device__ __forceinline__ bool next_for_one_thread(Shared& sh, Item& it) {  // the warp's other lanes have left
+        const int slot = count % RING;
+        if (!mbar_wait(&sh.item_full[slot], (uint32_t)(count / RING) & 1u)) return false;
+        it = sh.items[slot];
+        mbar_arrive(&sh.item_free[slot]);
+        ++count;
+        return true;
+    }
 };
 
 // Both streams on the same rows, tiles in turn.
 __device__ __forceinline__ bool shares_rows(const RaggedParams& p, const Item& it) { return it.ntok <= p.stream_tokens; }
+
+// Slots of key tile t behind the sequence's last key that a box brings all the same.
+__device__ __forceinline__ int dead_slots(const RaggedParams& p, const Item& it, int t) {
+    const int live = it.kv_total - t * BN;
+    return live < BN ? (live + p.box_rows - 1) / p.box_rows * p.box_rows - live : 0;
+}
 
 // Who reads a tile last: (stream, that stream's count of tiles) of the last three tiles, so that a producer knows which
 // barrier says that a ring slot is free.  MMAs of one thread retire in order, so the last reader speaks for both.
@@ -501,6 +516,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             mbar_init(&sh.item_full[i], 1);
             mbar_init(&sh.item_free[i], 11);  // every warp but the one that writes
         }
+        for (int i = 0; i < VS; ++i) mbar_init(&sh.v_patched[i], 1);
         mbar_init(&sh.part_bar, 8);
         mbar_init(&sh.flag_bar, 1);
         mbar_fence_init();
@@ -629,6 +645,18 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     }
                     walk.load(&tm_v, p, t, sV + (tiles % VS) * TILE_BYTES, &sh.v_full[tiles % VS]);
                     log.add(shared_rows, (t - it.kt0) & 1);
+                    // slots of the last box behind the sequence's last key may hold anything, and 0 * NaN is NaN
+                    const int dead = dead_slots(p, it, t), dead0 = it.kv_total - t * BN;
+                    if (dead) {
+                        alive = warp_wait(&sh.v_full[tiles % VS], (uint32_t)(tiles / VS) & 1u);
+                        for (int c = lane; c < dead * 16; c += 32)
+                            *reinterpret_cast<uint4*>(sV + (tiles % VS) * TILE_BYTES + ((c >> 3) & 1) * BLK_BYTES + (dead0 + (c >> 4)) * 128 +
+                                                      (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.v_patched[tiles % VS]);
+                        if (!alive) break;
+                    }
                 }
                 if (!alive) break;
             }
@@ -688,33 +716,30 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             constexpr uint32_t hi = umma_desc_hi(1024, UMMA_SW128);
             const uint32_t q_lo0 = umma_desc_lo(smem_u32(sQ), 16), k_lo0 = umma_desc_lo(smem_u32(sK), 16),
                            v_lo0 = umma_desc_lo(smem_u32(sV), BLK_BYTES);
-            int k_tiles = 0, v_tiles = 0;                // ring positions: tiles taken so far
-            int made0 = 0, made1 = 0, eaten0 = 0, eaten1 = 0;  // S and PV of each stream
-            int uses0 = 0, uses1 = 0;
-            while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
+            uint32_t k_tiles = 0, v_tiles = 0, patched = 0;        // tiles taken from the rings; parity of each V slot's patches
+            uint32_t made0 = 0, made1 = 0, eaten0 = 0, eaten1 = 0;  // S and PV of each stream
+            uint32_t uses0 = 0, uses1 = 0;
+            while (lane == 0 && (alive = reader.next_for_one_thread(sh, it)) && it.kt0 < it.kt1) {
                 const bool shared_rows = shares_rows(p, it);
                 const int per = shared_rows ? 1 : 2, steps = (it.kt1 - it.kt0) * per;  // step u: stream u % 2, tile u / per
-                alive = warp_wait(&sh.q_full[0], (uint32_t)uses0++ & 1u);
+                alive = mbar_wait(&sh.q_full[0], uses0++ & 1u);
                 auto scores = [&](int u) {  // S of step u
                     const int st = u & 1;
-                    if (!shared_rows && u == 1 && alive) alive = warp_wait(&sh.q_full[1], (uint32_t)uses1++ & 1u);
+                    if (!shared_rows && u == 1 && alive) alive = mbar_wait(&sh.q_full[1], uses1++ & 1u);
                     if (shared_rows || st == 0) {
-                        if (alive) alive = warp_wait(&sh.k_full[k_tiles % KS], (uint32_t)(k_tiles / KS) & 1u);
+                        if (alive) alive = mbar_wait(&sh.k_full[k_tiles % KS], (k_tiles / KS) & 1u);
                         ++k_tiles;
                     }
                     if (!alive) return;
-                    if (lane == 0) {
-                        const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
-                        const uint32_t k_lo = k_lo0 + (uint32_t)((k_tiles - 1) % KS) * (TILE_BYTES >> 4);
+                    const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
+                    const uint32_t k_lo = k_lo0 + ((k_tiles - 1) % KS) * (TILE_BYTES >> 4);
 #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
-                            umma_ss(tbase + COL_S + st * BN, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
-                        }
-                        tc_commit(&sh.s_full[st][(st ? made1 : made0) % SR]);
-                        if (u + (shared_rows ? 1 : 2) >= steps) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
+                    for (int kk = 0; kk < 8; ++kk) {
+                        const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
+                        umma_ss(tbase + COL_S + st * BN, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
                     }
-                    __syncwarp();
+                    tc_commit(&sh.s_full[st][(st ? made1 : made0) % SR]);
+                    if (u + per >= steps) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
                     if (st)
                         ++made1;
                     else
@@ -726,39 +751,33 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 for (int u = 0; u < steps && alive; ++u) {
                     const int st = u & 1, t = it.kt0 + (shared_rows ? u : u >> 1);
                     if (shared_rows || st == 0) {
-                        alive = warp_wait(&sh.v_full[v_tiles % VS], (uint32_t)(v_tiles / VS) & 1u);
+                        const uint32_t slot = v_tiles % VS;
+                        alive = mbar_wait(&sh.v_full[slot], (v_tiles / VS) & 1u);
                         ++v_tiles;
-                        if (!alive) break;
-                        // slots of the last box behind the sequence's last key may hold anything, and 0 * NaN is NaN
-                        const int dead0 = it.kv_total - t * BN, dead1 = min(BN, (dead0 + p.box_rows - 1) / p.box_rows * p.box_rows);
-                        if (dead0 < dead1) {
-                            for (int c = lane; c < (dead1 - dead0) * 16; c += 32)
-                                *reinterpret_cast<uint4*>(sV + ((v_tiles - 1) % VS) * TILE_BYTES + ((c >> 3) & 1) * BLK_BYTES +
-                                                          (dead0 + (c >> 4)) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                            fence_proxy_async_smem();
-                            __syncwarp();
+                        if (alive && dead_slots(p, it, t)) {
+                            alive = mbar_wait(&sh.v_patched[slot], (patched >> slot) & 1u);
+                            patched ^= 1u << slot;
                         }
+                        if (!alive) break;
                     }
-                    const uint32_t v_lo = v_lo0 + (uint32_t)((v_tiles - 1) % VS) * (TILE_BYTES >> 4);
+                    const uint32_t v_lo = v_lo0 + ((v_tiles - 1) % VS) * (TILE_BYTES >> 4);
                     const uint32_t p_col = tbase + COL_S + st * BN, o_col = tbase + COL_O + st * D;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {  // the halves of P arrive separately
-                        if (alive) alive = warp_wait(&sh.p_full[st][half], (uint32_t)(st ? eaten1 : eaten0) & 1u);
+                        if (alive) alive = mbar_wait(&sh.p_full[st][half], (st ? eaten1 : eaten0) & 1u);
                         if (!alive) break;
                         tc_fence_after();
-                        if (lane == 0) {
 #pragma unroll
-                            for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                                umma_ts(o_col, p_col + kk * 8, umma_desc_pack(v_lo + kk * (2048 >> 4), hi), idesc_o, kk > 0 || u > 1);
-                            if (half == 1) tc_commit(&sh.o_ready[st][(st ? eaten1 : eaten0) & 1]);
-                        }
-                        __syncwarp();
+                        for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                            umma_ts(o_col, p_col + kk * 8, umma_desc_pack(v_lo + kk * (2048 >> 4), hi), idesc_o, kk > 0 || u > 1);
                     }
+                    if (!alive) break;
+                    tc_commit(&sh.o_ready[st][(st ? eaten1 : eaten0) & 1]);
                     if (st)
                         ++eaten1;
                     else
                         ++eaten0;
-                    if (alive && u + 2 < steps) scores(u + 2);
+                    if (u + 2 < steps) scores(u + 2);
                 }
                 if (!alive) break;
             }
