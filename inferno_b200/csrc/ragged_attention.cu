@@ -45,8 +45,11 @@ namespace {
 constexpr int D = 128;
 constexpr int BM = 128, BN = RAGGED_TILE;
 constexpr int THREADS = 384;
-constexpr int KS = 3, VS = 2;          // tiles in the K and V rings
-constexpr int SR = 4;                  // rotation of the S barriers: a K slot is looked at up to KS - 1 tiles late
+#ifndef RKS
+#define RKS 3
+#endif
+constexpr int KS = RKS, VS = 5 - RKS;  // tiles in the K and V rings
+constexpr int SR = 4;                  // rotation of the barriers that free their slots: one is looked at up to three tiles late
 constexpr int TILE_BYTES = BN * D * 2;  // also the bytes of a stream's Q
 constexpr int BLK_BYTES = BN * 128;    // [128 rows][64 columns] with the 128-byte swizzle
 constexpr int RING = 4;                // item descriptions in flight
@@ -62,19 +65,26 @@ struct Item {
     int pieces, ordinal, group;    // of an item cut over several CTAs: how many, which one, the CTA of the first
 };
 
+struct Found {
+    long long at;  // where the sequence begins in the line
+    int b, n, past;
+};
+
 struct Shared {
     uint64_t q_full[2], q_free[2], k_full[KS], v_full[VS];
     uint64_t s_full[2][SR];   // S of a stream's tile is in TMEM, PV of its tile before has retired
     uint64_t p_full[2][2];    // keys 0-63 / 64-127 of a stream's P are in TMEM
-    uint64_t o_ready[2][2];   // PV of a stream's tile has retired
+    uint64_t o_ready[2][SR];  // PV of a stream's tile has retired
     uint64_t item_full[RING], item_free[RING];
     uint64_t v_patched[VS];   // dead slots of the V tile in this ring slot have been cleared
     uint64_t join[2];         // shared rows: stream 1's maxima and sums are in ml / its O has been read
-    uint64_t part_bar, flag_bar;  // a piece's rows are in scratch / whether it was the last
+    uint64_t part_bar, flag_bar;  // the CTA's pieces are in scratch / whether they were their items' last
     uint32_t tmem;
-    int last_piece;
+    int last_piece[2];
+    Item piece[2];                 // the CTA's pieces of cut items
     Item items[RING];
     long long scan[THREADS / 32];
+    Found found[2];                // the sequences that hold the part's ends
     int end[4], begin[4];          // (sequence, KV head, tile of tokens, key tile)
     int cut[2][3];                 // pieces, ordinal, group of the first and of the last item
     float ml[BM][2];
@@ -88,12 +98,12 @@ struct RaggedParams {
     const __half* q;
     const int *pages, *lens, *starts;
     int batch, max_pages, tokens, q_heads, kv_heads, group, page_size, num_pages, window;
-    int stream_tokens;  // Ts
+    int stream_tokens, few_tokens;  // tokens of a stream, and of an item of few rows at most
     int box_rows;       // keys of one TMA box
     float scale_log2;
     const float* gate;
     void* out;
-    int out_f16;
+    int out_f16, out_sectors;  // fp16 rows; rows begin at whole 32-byte sectors
     float *part_acc, *part_ml;  // [2 grid][256] rows
     int* counters;              // [grid], zero between launches
     int* status;
@@ -143,50 +153,100 @@ __device__ __forceinline__ T block_sum_before(T v, T& before, T* s_warp) {
     return total;
 }
 
-// Where CTA c's part of the line begins and ends.  Returns false where it has none.
+__device__ __forceinline__ RaggedHead head_of(const RaggedParams& p, int n, int past) {
+    return RaggedHead(n, past, 2 * p.stream_tokens, p.few_tokens, p.window);
+}
+
+// Where CTA c's part of the line begins and ends.  Returns false where it has none.  The threads sum the sequences' costs and
+// find the two sequences, then one warp each finds the place inside (read after the caller's barrier): its lanes take the
+// cuts that fall into the item, 32 at a time.
 __device__ __forceinline__ bool find_part(const RaggedParams& p, Shared& sh) {
     const int tid = threadIdx.x, c = blockIdx.x;
     const int per = (p.batch + THREADS - 1) / THREADS, b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
     int bad = 0;
     long long mine = 0, before;
+    Seq s{0, 0, 0};
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
-        const Seq s = sequence_of(p, b, bad);
-        mine += p.kv_heads * RaggedHead(s.n, s.past, 2 * p.stream_tokens, p.window).total();
+        s = sequence_of(p, b, bad);
+        mine += p.kv_heads * head_of(p, s.n, s.past).total();
     }
     if (bad && c == 0) atomicOr(p.status, bad);
-    if (tid == 0) {
-        sh.end[0] = p.batch;
-        sh.end[1] = sh.end[2] = sh.end[3] = 0;
-        sh.cut[1][0] = 1;
-    }
-    const long long total = block_sum_before(mine, before, sh.scan);
-    const int parts = ragged_parts(total, (int)gridDim.x);
-    if (c >= parts) return false;
-    const long long x[2] = {ragged_cut(total, parts, c), ragged_cut(total, parts, c + 1)};
-#pragma unroll
+    if (tid == 0) sh.found[1].b = p.batch;
+    const RaggedLine line(block_sum_before(mine, before, sh.scan), (int)gridDim.x);
+    if (c >= line.parts) return false;
+#pragma unroll 1
     for (int e = 0; e < 2; ++e) {
-        if (x[e] >= before && x[e] < before + mine) {
+        const long long x = line.cut(c + e);
+        if (x >= before && x < before + mine) {
             long long at = before;
-            for (int b = b0; b < b1; ++b) {
-                const Seq s = sequence_of(p, b, bad);
-                const RaggedHead h(s.n, s.past, 2 * p.stream_tokens, p.window);
-                const long long cost = p.kv_heads * h.total();
-                if (x[e] < at + cost) {
-                    int* out = e == 0 ? sh.begin : sh.end;
-                    out[0] = b;
-                    ragged_locate(h, at, x[e], total, parts, c, out + 1, sh.cut[e]);
-                    break;
-                }
+            int b = b0;
+            for (; per > 1; ++b) {
+                s = sequence_of(p, b, bad);
+                const long long cost = p.kv_heads * head_of(p, s.n, s.past).total();
+                if (x < at + cost) break;
                 at += cost;
             }
+            sh.found[e] = Found{at, b, s.n, s.past};
+        }
+    }
+    __syncthreads();
+    if (tid < 64) {
+        const int e = tid >> 5, lane = tid & 31;
+        const Found f = sh.found[e];
+        int* out = e == 0 ? sh.begin : sh.end;
+        int inside = 0, first = 0, tile = 0, kvh = 0, item = 0;
+        if (f.b < p.batch) {
+            const RaggedHead h = head_of(p, f.n, f.past);
+            const RaggedPlace place(h, f.at, line.cut(c + e));
+            kvh = place.kvh;
+            item = place.i;
+            const int first_tile = h.first_tile(item), end_tile = h.end_tile(item);
+            for (int k0 = place.first_cut(line);; k0 += 32) {
+                const int t = place.tile_of(h, line, k0 + lane);
+                const uint32_t in = __ballot_sync(0xffffffffu, t > first_tile && t < end_tile);
+                if (in && inside == 0) first = k0 + __ffs(in) - 1;
+                inside += __popc(in);
+                if (c + e >= k0 && c + e < k0 + 32) tile = __shfl_sync(0xffffffffu, t, c + e - k0);
+                if (__any_sync(0xffffffffu, t == end_tile)) break;  // these cuts reach the item's end
+            }
+        }
+        if (lane == 0) {
+            out[0] = f.b;
+            out[1] = kvh;
+            out[2] = item;
+            out[3] = tile;
+            sh.cut[e][0] = inside + 1;
+            sh.cut[e][1] = c - (first - 1);
+            sh.cut[e][2] = first - 1;
         }
     }
     return true;
 }
 
 // ---------------------------------------------------------------------------------------------- the kernel
-// A bounded wait of a whole warp, with one answer for all its lanes.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// A bounded wait in few instructions, because the code of the twelve warps has to fit the instruction caches: up to 2^21
+// tries of at most a microsecond each.
+__device__ __forceinline__ bool lone_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 tries;\n\t"
+        "mov.u32 tries, 0;\n"
+        "again:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "add.u32 tries, tries, 1;\n\t"
+        "setp.lt.u32 q, tries, 0x200000;\n\t"
+        "@p bra done;\n\t"
+        "@q bra again;\n"
+        "done:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// of a whole warp, with one answer for all its lanes
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, lone_wait(bar, parity)); }
 
 // A role's view of the items: the next one's description, copied to registers.
 struct ItemReader {
@@ -202,7 +262,7 @@ struct ItemReader {
     }
     __device__ __forceinline__ bool next_for_one_thread(Shared& sh, Item& it) {  // the warp's other lanes have left
         const int slot = count % RING;
-        if (!mbar_wait(&sh.item_full[slot], (uint32_t)(count / RING) & 1u)) return false;
+        if (!lone_wait(&sh.item_full[slot], (uint32_t)(count / RING) & 1u)) return false;
         it = sh.items[slot];
         mbar_arrive(&sh.item_free[slot]);
         ++count;
@@ -223,6 +283,7 @@ __device__ __forceinline__ int dead_slots(const RaggedParams& p, const Item& it,
 // barrier says that a ring slot is free.  MMAs of one thread retire in order, so the last reader speaks for both.
 struct TileLog {
     int cnt0 = 0, cnt1 = 0, back0 = 0, back1 = 0, back2 = 0;
+    __device__ __forceinline__ int back(int tiles) const { return tiles == 2 ? back1 : back2; }
     __device__ __forceinline__ void add(bool shared_rows, int turn) {
         back2 = back1;
         back1 = back0;
@@ -234,14 +295,25 @@ struct TileLog {
         }
     }
 };
-static_assert(KS == 3 && VS == 2, "back2 is the tile that a K slot held, back1 the tile that a V slot held");
+static_assert(KS >= 2 && KS <= 3 && VS >= 2 && VS <= 3, "the last three tiles are remembered");
+
+template <int N>
+struct RingPlace {
+    uint32_t slot = 0, parity = 0;
+    __device__ __forceinline__ void step() {
+        if (++slot == N) {
+            slot = 0;
+            parity ^= 1u;
+        }
+    }
+};
 
 // Row coordinates of the TMA boxes of 128 / box_rows tiles at a time, one box per lane, the next group looked up ahead.
 struct PageWalk {
     int per_tile, tiles;  // boxes per tile, tiles per group of 32 boxes
     int group = -1, y = 0, ahead = 0;
     __device__ __forceinline__ explicit PageWalk(const RaggedParams& p) : per_tile(BN / p.box_rows), tiles(32 / (BN / p.box_rows)) {}
-    __device__ __forceinline__ int lookup(const RaggedParams& p, const Item& it, int g, bool report) const {
+    __device__ __forceinline__ int lookup(const RaggedParams& p, const Item& it, int g) const {
         const int token = (g * tiles * BN) + (int)(threadIdx.x & 31) * p.box_rows;
         int row = p.num_pages * p.kv_heads * p.page_size;  // outside the tensor: zeros
         // boxes wholly below the lowest visible key may lie in pages that were given back
@@ -249,21 +321,21 @@ struct PageWalk {
             const int page = p.pages[(long long)it.b * p.max_pages + token / p.page_size];
             if (page >= 0 && page < p.num_pages)
                 row = (page * p.kv_heads + it.kvh) * p.page_size + token % p.page_size;
-            else if (report)
+            else
                 atomicOr(p.status, INF_STATUS_BAD_PAGE);
         }
         return row;
     }
-    __device__ __forceinline__ void begin(const RaggedParams& p, const Item& it, bool report) {
+    __device__ __forceinline__ void begin(const RaggedParams& p, const Item& it) {
         group = it.kt0 / tiles;
-        y = lookup(p, it, group, report);
-        ahead = lookup(p, it, group + 1, report);
+        y = lookup(p, it, group);
+        ahead = lookup(p, it, group + 1);
     }
-    __device__ __forceinline__ void step_to(const RaggedParams& p, const Item& it, int kt, bool report) {
+    __device__ __forceinline__ void step_to(const RaggedParams& p, const Item& it, int kt) {
         if (kt / tiles == group) return;
         group = kt / tiles;
         y = ahead;
-        ahead = lookup(p, it, group + 1, report);
+        ahead = lookup(p, it, group + 1);
     }
     // one [128 keys][128 dims] tile as two blocks of 64 columns; every lane issues its boxes
     __device__ __forceinline__ void load(const CUtensorMap* tm, const RaggedParams& p, int kt, uint8_t* dst, uint64_t* bar) const {
@@ -275,7 +347,7 @@ struct PageWalk {
     }
 };
 
-__device__ __forceinline__ bool few_rows(const RaggedParams& p, const Item& it) { return it.ntok * p.group <= FEW_ROWS; }
+__device__ __forceinline__ bool few_rows(const RaggedParams& p, const Item& it) { return it.ntok <= p.few_tokens; }
 
 // ---- one tile of a stream: S in TMEM -> P over it, and the row's running maximum and sum.  A row of O is scaled only when
 // its maximum grew by more than 2^8: until then the weights stay below 2^8.  Each row decides for itself, so that its bits do
@@ -294,10 +366,19 @@ __device__ __forceinline__ void exponentials(const uint32_t* x, float scale_log2
         packed[i / 2] = pack_half2(a, b);
     }
 }
-__device__ __forceinline__ void mask_keys(uint32_t* x, int k0, int qpos, int first_key) {
+// hides keys of a tile from a row: S is masked where it lies, so that the code below serves every tile
+__device__ __forceinline__ void mask_scores(uint32_t col_s, int k0, int qpos, int first_key) {
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+        uint32_t x[32];
+        tmem_ld32(col_s + c, x);
+        tc_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 64; ++i)
-        if (k0 + i > qpos || k0 + i < first_key) x[i] = 0xff800000u;  // -inf
+        for (int i = 0; i < 32; ++i)
+            if (k0 + c + i > qpos || k0 + c + i < first_key) x[i] = 0xff800000u;  // -inf
+        tmem_st32(col_s + c, x);
+    }
+    tc_wait_st();
 }
 __device__ __forceinline__ float max_of(const uint32_t* x) {
     float mx[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
@@ -309,59 +390,54 @@ __device__ __forceinline__ float max_of(const uint32_t* x) {
                 fmaxf(__uint_as_float(x[62]), __uint_as_float(x[63])));
 }
 
-// thread = row.  The weights of the first 64 keys are taken with the maximum so far while the rest of the row arrives and
-// its maximum is found; they are taken again (from S, which P has not covered yet) where that one turns out 2^8 larger.
+// thread = row.  Loops over the halves of the row, read from TMEM twice, keep the code short: three warps with different
+// code share a scheduler's instruction cache, and the thread that issues the MMAs must not wait for its instructions.
 __device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, uint32_t col_s, uint32_t col_o, int st, int k0,
                                              int qpos, int first_key, bool masked, bool valid, bool first, float& m_used, float& l) {
     const int lane = threadIdx.x & 31;
-    uint32_t x[BN], packed[32];
-    uint64_t sums[2] = {0, 0};
-    tmem_ld32(col_s, x);
-    tmem_ld32(col_s + 32, x + 32);
-    tc_wait_ld64(x);
-    tmem_ld32(col_s + 64, x + 64);
-    tmem_ld32(col_s + 96, x + 96);
-    if (masked) mask_keys(x, k0, qpos, first_key);
-    const float top0 = max_of(x);
-    if (!first) exponentials(x, p.scale_log2, m_used, packed, sums);
-    tc_wait_ld64(x + 64);
-    if (masked) mask_keys(x + 64, k0 + 64, qpos, first_key);
-    const float m_new = fmaxf(m_used, fmaxf(top0, max_of(x + 64)) * p.scale_log2);  // the scale is positive
-    const bool grew = first || (valid && m_new - m_used > RESCALE_THRESHOLD);
-    if (__any_sync(0xffffffffu, grew)) {
-        if (!first) {
-            const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
-            l *= alpha;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32(col_o + c * 32, o);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                tmem_st32(col_o + c * 32, o);
-            }
-            tc_wait_st();
-            tmem_ld32(col_s, x);
-            tmem_ld32(col_s + 32, x + 32);
-            tc_wait_ld64(x);
-            if (masked) mask_keys(x, k0, qpos, first_key);
-        }
-        m_used = grew ? m_new : m_used;
-        sums[0] = sums[1] = 0;
-        exponentials(x, p.scale_log2, m_used, packed, sums);
+    if (masked) mask_scores(col_s, k0, qpos, first_key);
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        uint32_t x[64];
+        tmem_ld32(col_s + h * 64, x);
+        tmem_ld32(col_s + h * 64 + 32, x + 32);
+        tc_wait_ld64(x);
+        top = fmaxf(top, max_of(x));
     }
-    tmem_st32(col_s, packed);
-    tc_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.p_full[st][0]);  // 64 keys of P are there: their PV may start
-    exponentials(x + 64, p.scale_log2, m_used, packed, sums);
-    tmem_st32(col_s + 32, packed);
-    tc_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.p_full[st][1]);
+    const float m_new = fmaxf(m_used, top * p.scale_log2);  // the scale is positive
+    const bool grew = valid && m_new - m_used > RESCALE_THRESHOLD;
+    if (first) {
+        m_used = m_new;
+    } else if (__any_sync(0xffffffffu, grew)) {
+        const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
+        m_used = grew ? m_new : m_used;
+        l *= alpha;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(col_o + c * 32, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(col_o + c * 32, o);
+        }
+        tc_wait_st();
+    }
+    uint64_t sums[2] = {0, 0};
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        uint32_t x[64], packed[32];
+        tmem_ld32(col_s + h * 64, x);
+        tmem_ld32(col_s + h * 64 + 32, x + 32);
+        tc_wait_ld64(x);
+        exponentials(x, p.scale_log2, m_used, packed, sums);
+        tmem_st32(col_s + h * 32, packed);  // over columns of S that have been read
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[st][h]);  // 64 keys of P are there: their PV may start
+    }
     float a, b;
     unpack_f32x2(add_f32x2(sums[0], sums[1]), a, b);
     l += a + b;
@@ -431,66 +507,100 @@ __device__ __forceinline__ void softmax_tile_few(Shared& sh, const RaggedParams&
     l += sum;
 }
 
+// 32 bytes of a thread's own row: one whole sector where the address allows it
+__device__ __forceinline__ void store_sector(void* at, const uint32_t* r, bool aligned) {
+    if (aligned) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                     "r"(r[5]), "r"(r[6]), "r"(r[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(at)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+        reinterpret_cast<uint4*>(at)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+    }
+}
+
 // ---- pieces of a cut item: row r of a stream of piece q in the scratch rows
 __device__ __forceinline__ long long piece_row(const Item& it, int q, int st, int r) {
     return ((long long)(q > 0 ? 2 * (it.group + q) : 2 * it.group + 1) * 2 + st) * BM + r;
 }
 
-// Joins the pieces in the order of the keys.  Each of the eight warps takes every eighth row: first lane = row (maxima, sums,
-// and each piece's weight, left in place of its maximum), then all lanes on one row's 128 values, four rows at a time so that
-// their loads overlap.
-__device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& it, int warp, int lane) {
-    __threadfence();
+// Joins the pieces in the order of the keys; `warps` warps take the rows in turn, ROWS of them with PIECES pieces each at a
+// time (32 loads of a row under way: the time is latency).
+template <int ROWS, int PIECES>
+__device__ __forceinline__ void join_rows(const RaggedParams& p, const Item& it, int warp, int warps, int lane) {
+    static_assert(ROWS * PIECES == 32, "a lane weighs one row's piece");
     const int per = p.stream_tokens * p.group, all = it.ntok * p.group;  // rows of a full stream, of the item
-    auto scratch_row = [&](int q, int rr) { return rr < per ? piece_row(it, q, 0, rr) : piece_row(it, q, 1, rr - per); };
-    auto out_row = [&](int rr) { return (long long)(it.tok0 + rr / p.group) * p.q_heads + it.kvh * p.group + rr % p.group; };
-    const int mine = warp + 8 * lane;
-    if (mine < all) {
+    auto row_in_piece = [&](int rr) { return rr < per ? rr : BM + rr - per; };
+#pragma unroll 1
+    for (int r0 = warp; r0 < all; r0 += ROWS * warps) {
+        // lane = (row, one of PIECES pieces); rows behind the last are read as the last and not stored
+        const int mine = min(r0 + lane / PIECES * warps, all - 1), q_mine = lane % PIECES;
+        const long long out_mine = (long long)(it.tok0 + mine / p.group) * p.q_heads + it.kvh * p.group + mine % p.group;
+        auto max_and_sum = [&](int q) {  // of one of this lane's pieces
+            return q < it.pieces ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + piece_row(it, q, 0, 0) + row_in_piece(mine))
+                                 : make_float2(M_INIT, 0.f);
+        };
         float m = M_INIT, sum = 0.f;
-        for (int q = 0; q < it.pieces; ++q) m = fmaxf(m, __ldcg(p.part_ml + scratch_row(q, mine) * 2));
-        for (int q = 0; q < it.pieces; ++q) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + scratch_row(q, mine));
-            sum = fmaf(ex2_approx(ml.x - m), ml.y, sum);
+#pragma unroll 1
+        for (int q = q_mine; q < it.pieces; q += PIECES) {
+            const float2 ml = max_and_sum(q);
+            const float m_new = fmaxf(m, ml.x);
+            sum = sum * ex2_approx(m - m_new) + ml.y * ex2_approx(ml.x - m_new);
+            m = m_new;
         }
-        float gain = 1.0f / sum;
-        if (p.gate) gain *= softplus(p.gate[out_row(mine)]);
-        for (int q = 0; q < it.pieces; ++q) {
-            float* at = p.part_ml + scratch_row(q, mine) * 2;
-            __stcg(at, ex2_approx(__ldcg(at) - m) * gain);
+#pragma unroll
+        for (int o = 1; o < PIECES; o <<= 1) {
+            const float m_other = __shfl_xor_sync(0xffffffffu, m, o), sum_other = __shfl_xor_sync(0xffffffffu, sum, o);
+            const float m_new = fmaxf(m, m_other);
+            sum = sum * ex2_approx(m - m_new) + sum_other * ex2_approx(m_other - m_new);
+            m = m_new;
         }
-    }
-    __syncwarp();
-    for (int r0 = warp; r0 < all; r0 += 32) {
-        float4 acc[4];
+        const float gain = (p.gate ? softplus(p.gate[out_mine]) : 1.0f) / sum;
+        float4 acc[ROWS];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-        for (int q = 0; q < it.pieces; ++q) {
+        for (int u = 0; u < ROWS; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int q = 0; q < it.pieces; q += PIECES) {
+            const float w = ex2_approx(max_and_sum(q + q_mine).x - m) * gain;  // 0 behind the last piece
+            float4 v[ROWS][PIECES];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (r0 + 8 * u < all) {
-                    const long long row = scratch_row(q, r0 + 8 * u);
-                    const float w = __ldcg(p.part_ml + row * 2);
-                    const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_acc + row * D) + lane);
-                    acc[u].x = fmaf(w, a.x, acc[u].x);
-                    acc[u].y = fmaf(w, a.y, acc[u].y);
-                    acc[u].z = fmaf(w, a.z, acc[u].z);
-                    acc[u].w = fmaf(w, a.w, acc[u].w);
+            for (int e = 0; e < PIECES; ++e) {
+                const float4* base = reinterpret_cast<const float4*>(p.part_acc + piece_row(it, min(q + e, it.pieces - 1), 0, 0) * D) + lane;
+#pragma unroll
+                for (int u = 0; u < ROWS; ++u) v[u][e] = __ldcg(base + row_in_piece(min(r0 + u * warps, all - 1)) * (D / 4));
+            }
+#pragma unroll
+            for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+                for (int e = 0; e < PIECES; ++e) {
+                    const float wu = __shfl_sync(0xffffffffu, w, u * PIECES + e);
+                    acc[u].x = fmaf(wu, v[u][e].x, acc[u].x);
+                    acc[u].y = fmaf(wu, v[u][e].y, acc[u].y);
+                    acc[u].z = fmaf(wu, v[u][e].z, acc[u].z);
+                    acc[u].w = fmaf(wu, v[u][e].w, acc[u].w);
                 }
-            }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (r0 + 8 * u < all) {
-                const long long row = out_row(r0 + 8 * u);
-                if (p.out_f16)
-                    reinterpret_cast<uint2*>((__half*)p.out + row * D)[lane] =
-                        make_uint2(pack_half2(acc[u].x, acc[u].y), pack_half2(acc[u].z, acc[u].w));
-                else
-                    reinterpret_cast<float4*>((float*)p.out + row * D)[lane] = acc[u];
-            }
+        for (int u = 0; u < ROWS; ++u) {
+            const long long row = __shfl_sync(0xffffffffu, out_mine, u * PIECES);
+            if (r0 + u * warps >= all) break;
+            if (p.out_f16)
+                reinterpret_cast<uint2*>((__half*)p.out + row * D)[lane] = make_uint2(pack_half2(acc[u].x, acc[u].y), pack_half2(acc[u].z, acc[u].w));
+            else
+                reinterpret_cast<float4*>((float*)p.out + row * D)[lane] = acc[u];
         }
     }
+}
+
+__device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& it, int warp, int warps, int lane) {
+    __threadfence();
+    // the order in which a row's sum is taken goes by its item alone, never by who joins it
+    if (it.pieces == 2)
+        join_rows<16, 2>(p, it, warp, warps, lane);
+    else if (it.ntok * p.group <= 16)  // a few rows a warp, as of decodes
+        join_rows<2, 16>(p, it, warp, warps, lane);
+    else
+        join_rows<8, 4>(p, it, warp, warps, lane);
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -505,18 +615,22 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], 1);
             mbar_init(&sh.q_free[i], 1);
-            for (int j = 0; j < SR; ++j) mbar_init(&sh.s_full[i][j], 1);
+            for (int j = 0; j < SR; ++j) {
+                mbar_init(&sh.s_full[i][j], 1);
+                mbar_init(&sh.o_ready[i][j], 1);
+            }
             for (int j = 0; j < 2; ++j) mbar_init(&sh.p_full[i][j], 4);  // one arrival per warp: tcgen05.wait is warp-wide
-            for (int j = 0; j < 2; ++j) mbar_init(&sh.o_ready[i][j], 1);
             mbar_init(&sh.join[i], 4);
         }
         for (int i = 0; i < KS; ++i) mbar_init(&sh.k_full[i], 1);
-        for (int i = 0; i < VS; ++i) mbar_init(&sh.v_full[i], 1);
+        for (int i = 0; i < VS; ++i) {
+            mbar_init(&sh.v_full[i], 1);
+            mbar_init(&sh.v_patched[i], 1);
+        }
         for (int i = 0; i < RING; ++i) {
             mbar_init(&sh.item_full[i], 1);
             mbar_init(&sh.item_free[i], 11);  // every warp but the one that writes
         }
-        for (int i = 0; i < VS; ++i) mbar_init(&sh.v_patched[i], 1);
         mbar_init(&sh.part_bar, 8);
         mbar_init(&sh.flag_bar, 1);
         mbar_fence_init();
@@ -566,7 +680,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 }
                 const int n = __shfl_sync(0xffffffffu, s.n, b - base), past = __shfl_sync(0xffffffffu, s.past, b - base),
                           start = __shfl_sync(0xffffffffu, s.start, b - base);
-                const RaggedHead h(n, past, 2 * p.stream_tokens, p.window);
+                const RaggedHead h = head_of(p, n, past);
                 if (i >= h.items) {
                     i = 0;
                     if (n == 0 || ++kvh >= p.kv_heads) {
@@ -603,12 +717,12 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     if (lane == 0) mbar_arrive(&sh.item_full[slot]);
                     ++items;
                     const bool shared_rows = shares_rows(p, it);
-                    walk.begin(p, it, true);
+                    walk.begin(p, it);
                     for (int t = it.kt0; t < it.kt1; ++t, ++tiles) {
-                        walk.step_to(p, it, t, true);
+                        walk.step_to(p, it, t);
                         if (tiles >= KS) {
-                            const int c = log.back2 >> 1;
-                            alive = warp_wait(&sh.s_full[log.back2 & 1][c % SR], (uint32_t)(c / SR) & 1u);
+                            const int who = log.back(KS), c = who >> 1;
+                            alive = warp_wait(&sh.s_full[who & 1][c % SR], (uint32_t)(c / SR) & 1u);
                             if (!alive) break;
                         }
                         walk.load(&tm_k, p, t, sK + (tiles % KS) * TILE_BYTES, &sh.k_full[tiles % KS]);
@@ -635,23 +749,23 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             PageWalk walk(p);
             while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
                 const bool shared_rows = shares_rows(p, it);
-                walk.begin(p, it, false);
+                walk.begin(p, it);
                 for (int t = it.kt0; t < it.kt1; ++t, ++tiles) {
-                    walk.step_to(p, it, t, false);
+                    walk.step_to(p, it, t);
                     if (tiles >= VS) {
-                        const int c = log.back1 >> 1;
-                        alive = warp_wait(&sh.o_ready[log.back1 & 1][c & 1], (uint32_t)(c >> 1) & 1u);
+                        const int who = log.back(VS), c = who >> 1;
+                        alive = warp_wait(&sh.o_ready[who & 1][c % SR], (uint32_t)(c / SR) & 1u);
                         if (!alive) break;
                     }
                     walk.load(&tm_v, p, t, sV + (tiles % VS) * TILE_BYTES, &sh.v_full[tiles % VS]);
                     log.add(shared_rows, (t - it.kt0) & 1);
                     // slots of the last box behind the sequence's last key may hold anything, and 0 * NaN is NaN
-                    const int dead = dead_slots(p, it, t), dead0 = it.kv_total - t * BN;
+                    const int dead = dead_slots(p, it, t);
                     if (dead) {
                         alive = warp_wait(&sh.v_full[tiles % VS], (uint32_t)(tiles / VS) & 1u);
+                        uint8_t* at = sV + (tiles % VS) * TILE_BYTES + (it.kv_total - t * BN) * 128;
                         for (int c = lane; c < dead * 16; c += 32)
-                            *reinterpret_cast<uint4*>(sV + (tiles % VS) * TILE_BYTES + ((c >> 3) & 1) * BLK_BYTES + (dead0 + (c >> 4)) * 128 +
-                                                      (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(at + ((c >> 3) & 1) * BLK_BYTES + (c >> 4) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sh.v_patched[tiles % VS]);
@@ -711,73 +825,82 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 }
             }
         } else {
-            // ------------------------------------------------ every MMA, from one thread
+            // ------------------------------------------------ every MMA, from one thread.  It runs about four MMAs (256
+            // cycles) ahead of the tensor cores; what it does between two groups must not take longer, so ring positions and
+            // parities are stepped, not computed, and the loop is short.
             constexpr uint32_t idesc_s = umma_idesc_f16(BM, BN, 0, 0), idesc_o = umma_idesc_f16(BM, D, 0, 1);
             constexpr uint32_t hi = umma_desc_hi(1024, UMMA_SW128);
             const uint32_t q_lo0 = umma_desc_lo(smem_u32(sQ), 16), k_lo0 = umma_desc_lo(smem_u32(sK), 16),
                            v_lo0 = umma_desc_lo(smem_u32(sV), BLK_BYTES);
-            uint32_t k_tiles = 0, v_tiles = 0, patched = 0;        // tiles taken from the rings; parity of each V slot's patches
-            uint32_t made0 = 0, made1 = 0, eaten0 = 0, eaten1 = 0;  // S and PV of each stream
-            uint32_t uses0 = 0, uses1 = 0;
+            RingPlace<KS> k_at;
+            RingPlace<VS> v_at;
+            RingPlace<SR> s_at[2], o_at[2];  // which barriers the next S and PV of a stream report to
+            uint32_t patched = 0, p_parity = 0, q_parity = 0;  // a bit for each V slot, stream, stream
             while (lane == 0 && (alive = reader.next_for_one_thread(sh, it)) && it.kt0 < it.kt1) {
                 const bool shared_rows = shares_rows(p, it);
-                const int per = shared_rows ? 1 : 2, steps = (it.kt1 - it.kt0) * per;  // step u: stream u % 2, tile u / per
-                alive = mbar_wait(&sh.q_full[0], uses0++ & 1u);
-                auto scores = [&](int u) {  // S of step u
-                    const int st = u & 1;
-                    if (!shared_rows && u == 1 && alive) alive = mbar_wait(&sh.q_full[1], uses1++ & 1u);
-                    if (shared_rows || st == 0) {
-                        if (alive) alive = mbar_wait(&sh.k_full[k_tiles % KS], (k_tiles / KS) & 1u);
-                        ++k_tiles;
-                    }
-                    if (!alive) return;
-                    const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
-                    const uint32_t k_lo = k_lo0 + ((k_tiles - 1) % KS) * (TILE_BYTES >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
-                        umma_ss(tbase + COL_S + st * BN, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
-                    }
-                    tc_commit(&sh.s_full[st][(st ? made1 : made0) % SR]);
-                    if (u + per >= steps) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
-                    if (st)
-                        ++made1;
-                    else
-                        ++made0;
-                };
-                scores(0);
-                if (steps > 1) scores(1);
+                const int steps = (it.kt1 - it.kt0) * (shared_rows ? 1 : 2);  // one tile of one stream each, the streams in turn
+                const int dead_step = dead_slots(p, it, it.kt1 - 1) ? (shared_rows ? steps - 1 : steps - 2) : -1;
+                uint32_t k_lo = 0, v_lo = 0;
+                alive = lone_wait(&sh.q_full[0], q_parity & 1u);
+                q_parity ^= 1u;
+                if (!shared_rows) {
+                    alive = alive && lone_wait(&sh.q_full[1], q_parity >> 1);
+                    q_parity ^= 2u;
+                }
+                // step w: PV of tile w - 2 of the steps, then S of tile w
 #pragma unroll 1
-                for (int u = 0; u < steps && alive; ++u) {
-                    const int st = u & 1, t = it.kt0 + (shared_rows ? u : u >> 1);
-                    if (shared_rows || st == 0) {
-                        const uint32_t slot = v_tiles % VS;
-                        alive = mbar_wait(&sh.v_full[slot], (v_tiles / VS) & 1u);
-                        ++v_tiles;
-                        if (alive && dead_slots(p, it, t)) {
-                            alive = mbar_wait(&sh.v_patched[slot], (patched >> slot) & 1u);
-                            patched ^= 1u << slot;
+                for (int w = 0; w < steps + 2; ++w) {
+                    const int st = w & 1;
+                    const uint32_t col_s = tbase + COL_S + st * BN, col_o = tbase + COL_O + st * D;
+                    const bool new_tile = shared_rows || st == 0;
+                    if (w >= 2) {
+                        if (new_tile) {
+                            alive = alive && lone_wait(&sh.v_full[v_at.slot], v_at.parity);
+                            if (w - 2 == dead_step) {
+                                alive = alive && lone_wait(&sh.v_patched[v_at.slot], (patched >> v_at.slot) & 1u);
+                                patched ^= 1u << v_at.slot;
+                            }
+                            v_lo = v_lo0 + v_at.slot * (TILE_BYTES >> 4);
+                            v_at.step();
+                        }
+#pragma unroll 1
+                        for (int half = 0; half < 2; ++half) {  // the halves of P arrive separately
+                            alive = alive && lone_wait(&sh.p_full[st][half], (p_parity >> st) & 1u);
+                            if (!alive) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk)
+                                umma_ts(col_o, col_s + half * 32 + kk * 8, umma_desc_pack(v_lo + (half * 4 + kk) * (2048 >> 4), hi), idesc_o,
+                                        kk > 0 || half > 0 || w >= 4);
                         }
                         if (!alive) break;
+                        p_parity ^= 1u << st;
+                        tc_commit(&sh.o_ready[st][st ? o_at[1].slot : o_at[0].slot]);
+                        if (st)
+                            o_at[1].step();
+                        else
+                            o_at[0].step();
                     }
-                    const uint32_t v_lo = v_lo0 + ((v_tiles - 1) % VS) * (TILE_BYTES >> 4);
-                    const uint32_t p_col = tbase + COL_S + st * BN, o_col = tbase + COL_O + st * D;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {  // the halves of P arrive separately
-                        if (alive) alive = mbar_wait(&sh.p_full[st][half], (st ? eaten1 : eaten0) & 1u);
+                    if (w < steps) {
+                        if (new_tile) {
+                            alive = alive && lone_wait(&sh.k_full[k_at.slot], k_at.parity);
+                            k_lo = k_lo0 + k_at.slot * (TILE_BYTES >> 4);
+                            k_at.step();
+                        }
                         if (!alive) break;
-                        tc_fence_after();
+                        const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
 #pragma unroll
-                        for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                            umma_ts(o_col, p_col + kk * 8, umma_desc_pack(v_lo + kk * (2048 >> 4), hi), idesc_o, kk > 0 || u > 1);
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
+                            umma_ss(col_s, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
+                        }
+                        tc_commit(&sh.s_full[st][st ? s_at[1].slot : s_at[0].slot]);
+                        if (st)
+                            s_at[1].step();
+                        else
+                            s_at[0].step();
+                        if (w + 1 == steps || (!shared_rows && w + 2 == steps)) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
                     }
-                    if (!alive) break;
-                    tc_commit(&sh.o_ready[st][(st ? eaten1 : eaten0) & 1]);
-                    if (st)
-                        ++eaten1;
-                    else
-                        ++eaten0;
-                    if (u + 2 < steps) scores(u + 2);
                 }
                 if (!alive) break;
             }
@@ -791,7 +914,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         const uint32_t col_s = tbase + lanes + COL_S + st * BN, col_o = tbase + lanes + COL_O + st * D;
         ItemReader reader;
         Item it;
-        int cnt = 0, joins = 0, parts_done = 0;  // tiles, items that both streams' rows were joined in, pieces
+        int cnt = 0, joins = 0, pieces = 0;  // tiles, items that both streams' rows were joined in, pieces of cut items
         bool ok = true;  // a wait that gave up: the rest runs through without waiting, so that nobody waits for this warp
         while (reader.next(sh, it) ? it.kt0 < it.kt1 : (ok = false)) {
             const bool shared_rows = shares_rows(p, it), few = few_rows(p, it);
@@ -821,7 +944,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 }
             }
             if (n > 0) {
-                if (ok) ok = warp_wait(&sh.o_ready[st][(cnt - 1) & 1], (uint32_t)((cnt - 1) >> 1) & 1u);
+                if (ok) ok = warp_wait(&sh.o_ready[st][(cnt - 1) % SR], (uint32_t)((cnt - 1) / SR) & 1u);
                 tc_fence_after();
             }
             if (few) {  // each thread of the quad has summed its own columns
@@ -895,7 +1018,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                             }
                         }
                     } else {
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             uint32_t o[32];
                             float y[32];
@@ -911,14 +1034,18 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                             }
                             if (valid && out16) {
 #pragma unroll
-                                for (int i = 0; i < 32; i += 8)
-                                    *reinterpret_cast<uint4*>(out16 + c * 32 + i) =
-                                        make_uint4(pack_half2(y[i], y[i + 1]), pack_half2(y[i + 2], y[i + 3]), pack_half2(y[i + 4], y[i + 5]),
-                                                   pack_half2(y[i + 6], y[i + 7]));
+                                for (int i = 0; i < 32; i += 16) {
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) o[e] = pack_half2(y[i + 2 * e], y[i + 2 * e + 1]);
+                                    store_sector(out16 + c * 32 + i, o, p.out_sectors);
+                                }
                             } else if (valid) {
 #pragma unroll
-                                for (int i = 0; i < 32; i += 4)
-                                    *reinterpret_cast<float4*>(out32 + c * 32 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                                for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(y[i + e]);
+                                    store_sector(out32 + c * 32 + i, o, p.out_sectors || cut);
+                                }
                             }
                             __syncwarp();
                         }
@@ -929,23 +1056,29 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 if (two && lane == 0) mbar_arrive(&sh.join[1]);
             }
             if (two) ++joins;
-            // ---- a cut item: whoever finishes its last piece joins the pieces in the order of the keys
             if (cut) {
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.part_bar);
-                if (ok) ok = warp_wait(&sh.part_bar, (uint32_t)parts_done & 1u);
-                if (tid == 0) {
-                    const int before = atomicAdd(&p.counters[it.group], 1);
-                    sh.last_piece = before + 1 == it.pieces;
-                    if (before + 1 == it.pieces) p.counters[it.group] = 0;  // for the next launch
-                    mbar_arrive(&sh.flag_bar);
-                }
-                __syncwarp();
-                if (ok) ok = warp_wait(&sh.flag_bar, (uint32_t)parts_done & 1u);
-                ++parts_done;
-                if (sh.last_piece) join_pieces(p, it, warp, lane);
+                if (tid == 0) sh.piece[pieces] = it;
+                ++pieces;
             }
+        }
+        // ---- cut items (the part's first and last at most): whoever finishes the last piece joins them in the order of the keys
+        if (pieces > 0) {
+            __threadfence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.part_bar);
+            if (ok) ok = warp_wait(&sh.part_bar, 0);
+            if (tid < pieces) {
+                const Item& mine = sh.piece[tid];
+                const int before = atomicAdd(&p.counters[mine.group], 1);
+                sh.last_piece[tid] = before + 1 == mine.pieces;
+                if (before + 1 == mine.pieces) p.counters[mine.group] = 0;  // for the next launch
+            }
+            __syncwarp();
+            if (tid == 0) mbar_arrive(&sh.flag_bar);
+            if (ok) ok = warp_wait(&sh.flag_bar, 0);
+            const bool one = sh.last_piece[0], other = pieces == 2 && sh.last_piece[1], both = one && other;
+            if (one || other)  // half of the warps each where there are two
+                join_pieces(p, sh.piece[both ? warp >> 2 : (one ? 0 : 1)], both ? warp & 3 : warp, both ? 4 : 8, lane);
         }
         if (!ok && lane == 0) atomicOr(p.status, INF_STATUS_WAIT_TIMEOUT);
     }
@@ -1021,12 +1154,14 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
         p.num_pages = pool->num_pages;
         p.window = sliding_window < table->max_pages * pool->page_size ? sliding_window : 0;  // a window no sequence can fill
         p.stream_tokens = BM / group;
+        p.few_tokens = FEW_ROWS / group;
         p.box_rows = 16;  // the widest box of whole pages' rows: a page holds a multiple of 16
         while (p.box_rows < BN && pool->page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;
         p.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)D)) * 1.4426950408889634f;
         p.gate = gate;
         p.out = out;
         p.out_f16 = out_dtype == INF_DTYPE_F16;
+        p.out_sectors = ((uintptr_t)out & 31u) == 0;
         p.status = ctx->status;
         const int grid = ctx->sm_count;
         rc = ragged_scratch(ctx, grid, &p.part_acc, &p.part_ml, &p.counters);
