@@ -503,7 +503,7 @@ int32_t inf_rope_append_gqa_ragged(inf_ctx* ctx, const void* q, const void* k, c
  * them, and their own keys and values have been appended at lens[b] onwards.  Row t sees keys [max(0, p + 1 - window), p],
  * p = lens[b] + t.  gate f32 [tokens][q_heads] (optional) applies softplus(gate); scale <= 0 means 1/sqrt(128); out
  * [tokens][q_heads][128] in out_dtype.  Rows from q_starts[batch] on are left as they were.  Up to 128 query heads per KV
- * head (INF_UNSUPPORTED beyond).  A sequence whose rows or length do not fit is skipped and reported, a page id outside
+ * head (INF_UNSUPPORTED beyond) and 2^29 tokens in a row of the page table.  A sequence whose rows or length do not fit is skipped and reported, a page id outside
  * the pool is reported and its keys read as zeros.  Keys and values of a sequence's tokens must be finite; pool slots behind
  * its last token may hold anything.  The context's first call allocates scratch (about 40 MB); make it before a capture.
  * Calls of one context, and graphs captured through it, share that scratch and must not overlap on the GPU: work that runs

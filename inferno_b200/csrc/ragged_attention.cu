@@ -524,36 +524,37 @@ __device__ __forceinline__ long long piece_row(const Item& it, int q, int st, in
     return ((long long)(q > 0 ? 2 * (it.group + q) : 2 * it.group + 1) * 2 + st) * BM + r;
 }
 
-// Joins the pieces in the order of the keys; `warps` warps take the rows in turn, ROWS of them with PIECES pieces each at a
-// time (32 loads of a row under way: the time is latency).
-template <int ROWS, int PIECES>
-__device__ __forceinline__ void join_rows(const RaggedParams& p, const Item& it, int warp, int warps, int lane) {
-    static_assert(ROWS * PIECES == 32, "a lane weighs one row's piece");
+// Joins the pieces in the order of the keys; `warps` warps take the rows in turn, eight of them with four pieces each at a
+// time: the time is latency, so what counts is how many loads are under way.
+__device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& it, int warp, int warps, int lane) {
+    constexpr int ROWS = 8, PIECES = 4;
+    __threadfence();
     const int per = p.stream_tokens * p.group, all = it.ntok * p.group;  // rows of a full stream, of the item
     auto row_in_piece = [&](int rr) { return rr < per ? rr : BM + rr - per; };
 #pragma unroll 1
     for (int r0 = warp; r0 < all; r0 += ROWS * warps) {
-        // lane = (row, one of PIECES pieces); rows behind the last are read as the last and not stored
-        const int mine = min(r0 + lane / PIECES * warps, all - 1), q_mine = lane % PIECES;
+        // lane = (row, one of four pieces); rows behind the last are read as the last and not stored
+        const int mine = min(r0 + lane / PIECES * warps, all - 1);
         const long long out_mine = (long long)(it.tok0 + mine / p.group) * p.q_heads + it.kvh * p.group + mine % p.group;
         auto max_and_sum = [&](int q) {  // of one of this lane's pieces
             return q < it.pieces ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + piece_row(it, q, 0, 0) + row_in_piece(mine))
                                  : make_float2(M_INIT, 0.f);
         };
+        auto merge = [](float& m, float& sum, float m2, float sum2) {
+            const float top = fmaxf(m, m2);
+            sum = sum * ex2_approx(m - top) + sum2 * ex2_approx(m2 - top);
+            m = top;
+        };
         float m = M_INIT, sum = 0.f;
 #pragma unroll 1
-        for (int q = q_mine; q < it.pieces; q += PIECES) {
+        for (int q = lane % PIECES; q < it.pieces; q += PIECES) {
             const float2 ml = max_and_sum(q);
-            const float m_new = fmaxf(m, ml.x);
-            sum = sum * ex2_approx(m - m_new) + ml.y * ex2_approx(ml.x - m_new);
-            m = m_new;
+            merge(m, sum, ml.x, ml.y);
         }
 #pragma unroll
         for (int o = 1; o < PIECES; o <<= 1) {
-            const float m_other = __shfl_xor_sync(0xffffffffu, m, o), sum_other = __shfl_xor_sync(0xffffffffu, sum, o);
-            const float m_new = fmaxf(m, m_other);
-            sum = sum * ex2_approx(m - m_new) + sum_other * ex2_approx(m_other - m_new);
-            m = m_new;
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
+            merge(m, sum, m2, sum2);
         }
         const float gain = (p.gate ? softplus(p.gate[out_mine]) : 1.0f) / sum;
         float4 acc[ROWS];
@@ -561,24 +562,29 @@ __device__ __forceinline__ void join_rows(const RaggedParams& p, const Item& it,
         for (int u = 0; u < ROWS; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
         for (int q = 0; q < it.pieces; q += PIECES) {
-            const float w = ex2_approx(max_and_sum(q + q_mine).x - m) * gain;  // 0 behind the last piece
-            float4 v[ROWS][PIECES];
+            const float w = ex2_approx(max_and_sum(q + lane % PIECES).x - m) * gain;  // 0 behind the last piece
+            float4 v[PIECES][ROWS];
 #pragma unroll
             for (int e = 0; e < PIECES; ++e) {
-                const float4* base = reinterpret_cast<const float4*>(p.part_acc + piece_row(it, min(q + e, it.pieces - 1), 0, 0) * D) + lane;
+                if (q + e < it.pieces) {
+                    const float4* base = reinterpret_cast<const float4*>(p.part_acc + piece_row(it, q + e, 0, 0) * D) + lane;
 #pragma unroll
-                for (int u = 0; u < ROWS; ++u) v[u][e] = __ldcg(base + row_in_piece(min(r0 + u * warps, all - 1)) * (D / 4));
+                    for (int u = 0; u < ROWS; ++u) v[e][u] = __ldcg(base + row_in_piece(min(r0 + u * warps, all - 1)) * (D / 4));
+                }
             }
 #pragma unroll
-            for (int u = 0; u < ROWS; ++u)
+            for (int e = 0; e < PIECES; ++e) {
+                if (q + e < it.pieces) {
 #pragma unroll
-                for (int e = 0; e < PIECES; ++e) {
-                    const float wu = __shfl_sync(0xffffffffu, w, u * PIECES + e);
-                    acc[u].x = fmaf(wu, v[u][e].x, acc[u].x);
-                    acc[u].y = fmaf(wu, v[u][e].y, acc[u].y);
-                    acc[u].z = fmaf(wu, v[u][e].z, acc[u].z);
-                    acc[u].w = fmaf(wu, v[u][e].w, acc[u].w);
+                    for (int u = 0; u < ROWS; ++u) {
+                        const float wu = __shfl_sync(0xffffffffu, w, u * PIECES + e);
+                        acc[u].x = fmaf(wu, v[e][u].x, acc[u].x);
+                        acc[u].y = fmaf(wu, v[e][u].y, acc[u].y);
+                        acc[u].z = fmaf(wu, v[e][u].z, acc[u].z);
+                        acc[u].w = fmaf(wu, v[e][u].w, acc[u].w);
+                    }
                 }
+            }
         }
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) {
@@ -590,17 +596,6 @@ __device__ __forceinline__ void join_rows(const RaggedParams& p, const Item& it,
                 reinterpret_cast<float4*>((float*)p.out + row * D)[lane] = acc[u];
         }
     }
-}
-
-__device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& it, int warp, int warps, int lane) {
-    __threadfence();
-    // the order in which a row's sum is taken goes by its item alone, never by who joins it
-    if (it.pieces == 2)
-        join_rows<16, 2>(p, it, warp, warps, lane);
-    else if (it.ntok * p.group <= 16)  // a few rows a warp, as of decodes
-        join_rows<2, 16>(p, it, warp, warps, lane);
-    else
-        join_rows<8, 4>(p, it, warp, warps, lane);
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -1122,8 +1117,8 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
             return inf_fail(ctx, INF_E_CACHE, "%s: page_size must be a positive multiple of 16, got %d", what, pool->page_size);
         if ((long long)pool->num_pages * pool->kv_heads * pool->page_size >= 0x7fffffffLL)
             return inf_fail(ctx, INF_E_CACHE, "%s: the pool's rows must be countable in 31 bits", what);
-        if ((long long)table->max_pages * pool->page_size > (1LL << 30))
-            return inf_fail(ctx, INF_E_CACHE, "%s: a page-table row must not hold more than 2^30 tokens", what);
+        if ((long long)table->max_pages * pool->page_size > (1LL << 29))
+            return inf_fail(ctx, INF_E_CACHE, "%s: a page-table row must not hold more than 2^29 tokens", what);
         if (tokens < 0) return inf_fail(ctx, INF_E_SHAPE, "%s: tokens must not be negative", what);
         if (q_heads <= 0 || q_heads % pool->kv_heads != 0)
             return inf_fail(ctx, INF_E_SHAPE, "%s: q_heads %d must be a positive multiple of kv_heads %d", what, q_heads, pool->kv_heads);

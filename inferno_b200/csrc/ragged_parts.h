@@ -9,16 +9,18 @@
 #endif
 
 constexpr int RAGGED_TILE = 128;  // keys of a tile
-// Costs, in halves of a key of an item of few rows.  A key of an item of two streams costs twice, of one stream of many rows
-// one and a half times as much; an item costs some keys besides; and a CTA's part is worth three tiles at least, which also
+// Costs, in halves of a key of an item of few rows.  A key of an item of two streams costs two and a half times, of one
+// stream of many rows one and a half times as much (with twice instead: two chunks of 1 024 among 46 decodes 172 us, now 160;
+// a window of 512 47 us, now 49); an item costs some keys besides; and a CTA's part is worth three tiles at least, which also
 // keeps two cuts of one item from falling on the same tile.
 constexpr int RAGGED_ITEM_COST = 512;
 constexpr int RAGGED_MIN_PART = 2 * 3 * RAGGED_TILE;
 constexpr int RAGGED_SNAP = 2;
 
-// The items of T tokens of one KV head of a sequence: n new tokens behind `past` cached ones, past + n at most 2^30.  An item
+// The items of T tokens of one KV head of a sequence: n new tokens behind `past` cached ones, past + n at most 2^29.  An item
 // of more than T / 2 tokens has two streams, one of up to `few` tokens few rows.
 struct RaggedHead {
+    enum { PAIR = 5 };
     int n, past, T, few, window, items;
     RAGGED_FN RaggedHead(int n_, int past_, int T_, int few_, int window_)
         : n(n_), past(past_), T(T_), few(few_), window(window_), items((int)((unsigned)(n_ + T_ - 1) / (unsigned)T_)) {}
@@ -31,7 +33,7 @@ struct RaggedHead {
     RAGGED_FN int end_tile(int i) const { return (hi(i) + RAGGED_TILE - 1) / RAGGED_TILE; }
     RAGGED_FN int weight(int i) const {
         const int tokens = n - i * T;
-        return tokens > T / 2 ? 4 : (tokens > few ? 3 : 2);
+        return tokens > T / 2 ? PAIR : (tokens > few ? 3 : 2);
     }
     RAGGED_FN long long cost(int i) const { return RAGGED_ITEM_COST + (long long)weight(i) * (hi(i) - lo(i)); }
     // cost of the items before item i (all of T tokens): past + (i + 1) T keys each, or T + window - 1 where the window bites
@@ -39,7 +41,7 @@ struct RaggedHead {
         int m = i;  // items that the window does not reach
         if (window > 0) m = least(m, (int)((unsigned)most(0, T + window - 1 - past) / (unsigned)T));
         const long long keys = (long long)m * past + (long long)T * (((long long)m * (m + 1)) >> 1) + (long long)(i - m) * (T + window - 1);
-        return (long long)i * RAGGED_ITEM_COST + 4 * keys;
+        return (long long)i * RAGGED_ITEM_COST + PAIR * keys;
     }
     RAGGED_FN long long total() const { return items > 0 ? before(items - 1) + cost(items - 1) : 0; }
     RAGGED_FN int item_at(long long y) const {  // largest i with before(i) <= y
@@ -56,11 +58,10 @@ struct RaggedHead {
     // The key tile at which a cut z into the cost of item i falls.  A cut within RAGGED_SNAP tiles of an end of an item of two
     // streams goes there: the pieces of up to 256 rows cost more than so many tiles.
     RAGGED_FN int tile_at(int i, long long z) const {
-        const int first = first_tile(i), end = end_tile(i), w = weight(i), snap = w == 4 ? RAGGED_SNAP : 0;
+        const int first = first_tile(i), end = end_tile(i), w = weight(i), snap = w == PAIR ? RAGGED_SNAP : 0;
         if (z <= RAGGED_ITEM_COST) return first;
-        const unsigned past_fixed = (unsigned)(z - RAGGED_ITEM_COST);
-        const unsigned keys = w == 3 ? past_fixed / 3u : past_fixed >> (w >> 1);
-        const int tile = (int)(((unsigned)lo(i) + keys + RAGGED_TILE / 2) / RAGGED_TILE);
+        const unsigned past_fixed = (unsigned)(z - RAGGED_ITEM_COST);  // below 5 * 2^29
+        const int tile = (int)(((unsigned)lo(i) + past_fixed / (unsigned)w + RAGGED_TILE / 2) / RAGGED_TILE);
         if (tile <= first + snap) return first;
         return tile >= end - snap ? end : tile;
     }

@@ -139,7 +139,7 @@ def test_every_tile_is_taken_once(check, seed):
               rng.choice([0, 1, 10]))
 
 
-@pytest.mark.parametrize("past,new", [([1 << 29], [1]), ([(1 << 30) - 300], [300]), ([0], [1 << 20]), ([0, 0], [0, 0])])
+@pytest.mark.parametrize("past,new", [([(1 << 29) - 1], [1]), ([(1 << 29) - 300], [300]), ([0], [1 << 20]), ([0, 0], [0, 0])])
 def test_extremes(check, past, new):
     check(past, new, 8 if new[0] < 1000 else 1, 42, 0, 148)
     check(past, new, 8 if new[0] < 1000 else 1, 42, 512, 148)
