@@ -54,6 +54,7 @@ constexpr int TILE_BYTES = BN * D * 2;  // also the bytes of a stream's Q
 constexpr int BLK_BYTES = BN * 128;    // [128 rows][64 columns] with the 128-byte swizzle
 constexpr int RING = 4;                // item descriptions in flight
 constexpr int FEW_ROWS = 32;           // rows that are dealt out to the lane quarters, eight each
+constexpr int LIGHT_ROWS = 64;         // rows up to which an item's time is that of its keys' way from memory
 constexpr float M_INIT = -1.0e30f;
 constexpr float RESCALE_THRESHOLD = 8.0f;
 constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;  // 128 columns per stream each
@@ -98,7 +99,8 @@ struct RaggedParams {
     const __half* q;
     const int *pages, *lens, *starts;
     int batch, max_pages, tokens, q_heads, kv_heads, group, page_size, num_pages, window;
-    int stream_tokens, few_tokens;  // tokens of a stream, and of an item of few rows at most
+    int stream_tokens;              // Ts
+    int few_tokens, light_tokens;   // of an item of FEW_ROWS / LIGHT_ROWS rows at most
     int box_rows;       // keys of one TMA box
     float scale_log2;
     const float* gate;
@@ -154,7 +156,7 @@ __device__ __forceinline__ T block_sum_before(T v, T& before, T* s_warp) {
 }
 
 __device__ __forceinline__ RaggedHead head_of(const RaggedParams& p, int n, int past) {
-    return RaggedHead(n, past, 2 * p.stream_tokens, p.few_tokens, p.window);
+    return RaggedHead(n, past, 2 * p.stream_tokens, p.light_tokens, p.window);
 }
 
 // Where CTA c's part of the line begins and ends.  Returns false where it has none.  The threads sum the sequences' costs and
@@ -1150,6 +1152,7 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
         p.window = sliding_window < table->max_pages * pool->page_size ? sliding_window : 0;  // a window no sequence can fill
         p.stream_tokens = BM / group;
         p.few_tokens = FEW_ROWS / group;
+        p.light_tokens = LIGHT_ROWS / group;
         p.box_rows = 16;  // the widest box of whole pages' rows: a page holds a multiple of 16
         while (p.box_rows < BN && pool->page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;
         p.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)D)) * 1.4426950408889634f;

@@ -9,21 +9,22 @@
 #endif
 
 constexpr int RAGGED_TILE = 128;  // keys of a tile
-// Costs, in halves of a key of an item of few rows.  A key of an item of two streams costs two and a half times, of one
-// stream of many rows one and a half times as much (with twice instead: two chunks of 1 024 among 46 decodes 172 us, now 160;
-// a window of 512 47 us, now 49); an item costs some keys besides; and a CTA's part is worth three tiles at least, which also
-// keeps two cuts of one item from falling on the same tile.
+// Costs, in halves of a key of a light item.  A key of an item of two streams costs two and a half times as much (with twice:
+// two chunks of 1 024 among 46 decodes 172 us, now 160; a window of 512 47 us, now 49), of one stream of many rows one and a
+// half times (items of 33 to 64 rows count as light: 24 sequences' drafts 95 us as heavy ones, now 82); an item costs some
+// keys besides; and a CTA's part is worth three tiles at least, which also keeps two cuts of one item from falling on the
+// same tile.
 constexpr int RAGGED_ITEM_COST = 512;
 constexpr int RAGGED_MIN_PART = 2 * 3 * RAGGED_TILE;
 constexpr int RAGGED_SNAP = 2;
 
 // The items of T tokens of one KV head of a sequence: n new tokens behind `past` cached ones, past + n at most 2^29.  An item
-// of more than T / 2 tokens has two streams, one of up to `few` tokens few rows.
+// of more than T / 2 tokens has two streams, one of up to `light` tokens is light.
 struct RaggedHead {
     enum { PAIR = 5 };
-    int n, past, T, few, window, items;
-    RAGGED_FN RaggedHead(int n_, int past_, int T_, int few_, int window_)
-        : n(n_), past(past_), T(T_), few(few_), window(window_), items((int)((unsigned)(n_ + T_ - 1) / (unsigned)T_)) {}
+    int n, past, T, light, window, items;
+    RAGGED_FN RaggedHead(int n_, int past_, int T_, int light_, int window_)
+        : n(n_), past(past_), T(T_), light(light_), window(window_), items((int)((unsigned)(n_ + T_ - 1) / (unsigned)T_)) {}
     RAGGED_FN static int least(int a, int b) { return a < b ? a : b; }
     RAGGED_FN static int most(int a, int b) { return a > b ? a : b; }
     // keys [lo, hi) that some row of item i sees
@@ -33,7 +34,7 @@ struct RaggedHead {
     RAGGED_FN int end_tile(int i) const { return (hi(i) + RAGGED_TILE - 1) / RAGGED_TILE; }
     RAGGED_FN int weight(int i) const {
         const int tokens = n - i * T;
-        return tokens > T / 2 ? PAIR : (tokens > few ? 3 : 2);
+        return tokens > T / 2 ? PAIR : (tokens > light ? 3 : 2);
     }
     RAGGED_FN long long cost(int i) const { return RAGGED_ITEM_COST + (long long)weight(i) * (hi(i) - lo(i)); }
     // cost of the items before item i (all of T tokens): past + (i + 1) T keys each, or T + window - 1 where the window bites
