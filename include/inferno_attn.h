@@ -463,7 +463,7 @@ int32_t inf_linearize_paged(inf_ctx* ctx, const void* pool_f16, const inf_kv_poo
 
 /* inf_paged_index on the GPU: caller-owned int32 arrays.  Slots of `pages` below ceil(lens[b] / page_size) hold page ids;
  * the free list is a stack, free_pages[0 .. *free_count).  num_pages * page_size and max_pages * page_size must fit 31
- * bits.  One call at a time may work on an index. */
+ * bits, and max_seqs is at most 16384.  One call at a time may work on an index. */
 typedef struct inf_device_index {
     int32_t* pages;      /* [max_seqs][max_pages] */
     int32_t* lens;       /* [max_seqs] tokens cached */

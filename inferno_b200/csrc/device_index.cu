@@ -7,12 +7,21 @@
 // pages in the reverse order (the last sequence's last page first), so an append followed by a truncate to the old
 // lengths restores the free list exactly.  Both are prefix sums over the batch; a few KB move, so what counts is the
 // length of the chain of dependent loads.
+//
+// A cluster of up to eight CTAs shares a call.  Each takes the prefix sums over the whole batch into its own shared
+// memory, which is cheaper than waiting for another's, and then its share of the tokens and of the pages:
+// a search of the prefix sums gives the sequence, and a fresh page is read from the free list itself, not from the row
+// that another thread is writing.  The cluster's barrier stands between the last read of the lengths and their update.
+// An append and a truncate in a graph take 8.2 us for 32 decodes, 11.0 for 300 sequences of up to 9 new tokens, and 19.1
+// for 1000 of up to 127 (65 000 rows; one CTA alone: 94), of which the two launches are about 5.
 #include "common.cuh"
 
 namespace {
 
 constexpr int THREADS = 1024;
 constexpr int WARPS = THREADS / 32;
+constexpr int MOST_CTAS = 8;
+constexpr int MOST_SEQS = 16384;  // three words of shared memory each
 
 struct IndexArgs {
     int* pages;
@@ -23,155 +32,230 @@ struct IndexArgs {
     int* status;
 };
 
-// Sum over the block of one value per thread and, per thread, the sum over the threads before it.
-__device__ __forceinline__ long long block_scan(long long v, long long& before, long long* s_warp) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ int cluster_rank() {
+    int r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// Replaces x[0 .. n) by the sums of the values before them and writes the whole sum to x[n]; y likewise if given.  The
+// sums themselves (returned) are taken in 64 bits.  A thread takes ceil(n / THREADS) neighbours.
+struct Sums {
+    long long x, y;
+};
+__device__ __forceinline__ Sums prefix_sums(int* x, int* y, int n, Sums* s_warp) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long inc = v;
+    const int each = (n + THREADS - 1) / THREADS, from = min((int)threadIdx.x * each, n), to = min(from + each, n);
+    Sums mine{0, 0};
+    for (int i = from; i < to; ++i) {
+        mine.x += x[i];
+        if (y) mine.y += y[i];
+    }
+    Sums inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
+        const long long ux = __shfl_up_sync(0xffffffffu, inc.x, o);
+        if (lane >= o) inc.x += ux;
+        if (y) {
+            const long long uy = __shfl_up_sync(0xffffffffu, inc.y, o);
+            if (lane >= o) inc.y += uy;
+        }
     }
-    __syncthreads();  // the warp sums of the call before this one have been read
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    long long base = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        const long long x = s_warp[w];
-        if (w < warp) base += x;
-        total += x;
+    Sums base{0, 0}, total{0, 0};
+    const int used = (n + 32 * each - 1) / (32 * each);  // warps that hold values
+    for (int w = 0; w < used; ++w) {
+        const Sums v = s_warp[w];
+        if (w < warp) base.x += v.x, base.y += v.y;
+        total.x += v.x, total.y += v.y;
     }
-    before = base + inc - v;
+    Sums run{base.x + inc.x - mine.x, base.y + inc.y - mine.y};
+    for (int i = from; i < to; ++i) {
+        const int vx = x[i];
+        x[i] = (int)run.x;
+        run.x += vx;
+        if (y) {
+            const int vy = y[i];
+            y[i] = (int)run.y;
+            run.y += vy;
+        }
+    }
+    if (threadIdx.x == 0) {
+        x[n] = (int)total.x;
+        if (y) y[n] = (int)total.y;
+    }
+    __syncthreads();
     return total;
+}
+
+// The last i of [0, n) with sums[i] <= v, for sums[0] <= v < sums[n]: its own value is not zero.
+__device__ __forceinline__ int holder_of(const int* sums, int n, int v) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] <= v)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
 }
 
 __device__ __forceinline__ int pages_of(long long tokens, int page_size) { return (int)((tokens + page_size - 1) / page_size); }
 
+// A thread takes EACH neighbouring tokens at a time: one while the cluster has a thread for every token, four (one search,
+// 16-byte stores) when it has not.
+template <int EACH>
 __global__ void __launch_bounds__(THREADS)
 device_index_append_kernel(IndexArgs a, const int* __restrict__ new_tokens, int max_tokens, int* __restrict__ past_lens,
                            int* __restrict__ q_starts, int* __restrict__ positions, int* __restrict__ slots) {
-    __shared__ long long s_warp[WARPS];
+    __shared__ Sums s_warp[WARPS];
+    extern __shared__ int s_seqs[];
+    int *s_past = s_seqs, *s_start = s_past + a.seqs, *s_fresh = s_start + a.seqs + 1;
     inf_pdl_wait();
     inf_pdl_release();
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, rank = cluster_rank(), i0 = rank * THREADS + tid, stride = (int)gridDim.x * THREADS;
     const long long capacity = (long long)a.max_pages * a.page_size;
     const int free_count = *a.free_count;
     // ---- a step that does not fit is refused as a whole, before anything of the index changes
     int bad = free_count < 0 || free_count > a.num_pages ? INF_STATUS_NO_PAGES : 0;
-    long long tokens = 0, need = 0;
     for (int b = tid; b < a.seqs; b += THREADS) {
         const int past = a.lens[b], n = new_tokens[b];
-        if (past < 0 || n < 0 || (long long)past + n > capacity) {
-            bad |= INF_STATUS_BAD_LEN;
-        } else {
-            tokens += n;
-            need += pages_of((long long)past + n, a.page_size) - pages_of(past, a.page_size);
-        }
+        const bool fits = past >= 0 && n >= 0 && (long long)past + n <= capacity;
+        if (!fits) bad |= INF_STATUS_BAD_LEN;
+        s_past[b] = past;
+        s_start[b] = fits ? n : 0;
+        s_fresh[b] = fits ? pages_of((long long)past + n, a.page_size) - pages_of(past, a.page_size) : 0;
     }
-    long long unused;
-    const long long total = block_scan(tokens, unused, s_warp);
-    const long long fresh_total = block_scan(need, unused, s_warp);
-    if (total > max_tokens) bad |= INF_STATUS_BAD_LEN;
-    if (fresh_total > free_count) bad |= INF_STATUS_NO_PAGES;
-    if (__syncthreads_or(bad)) {
-        if (bad) atomicOr(a.status, bad);
-        for (int b = tid; b < a.seqs; b += THREADS) past_lens[b] = a.lens[b];
-        for (int b = tid; b <= a.seqs; b += THREADS) q_starts[b] = 0;
-        for (int t = tid; t < max_tokens; t += THREADS) positions[t] = slots[t] = -1;
+    const bool any_bad = __syncthreads_or(bad);
+    cluster_arrive();  // this CTA has read the lengths and the count
+    const Sums total = prefix_sums(s_start, s_fresh, a.seqs, s_warp);
+    if (total.x > max_tokens) bad |= INF_STATUS_BAD_LEN;
+    if (total.y > free_count) bad |= INF_STATUS_NO_PAGES;
+    if (any_bad || total.x > max_tokens || total.y > free_count) {
+        if (bad && rank == 0) atomicOr(a.status, bad);
+        for (int b = i0; b < a.seqs; b += stride) past_lens[b] = s_past[b];
+        for (int b = i0; b <= a.seqs; b += stride) q_starts[b] = 0;
+        for (int t = i0; t < max_tokens; t += stride) positions[t] = slots[t] = -1;
+        cluster_wait();
         return;
     }
-    // ---- pages and starts, a block of sequences at a time
-    long long token0 = 0, page0 = 0;
-    for (int b0 = 0; b0 < a.seqs; b0 += THREADS) {
-        const int b = b0 + tid;
-        const int past = b < a.seqs ? a.lens[b] : 0, n = b < a.seqs ? new_tokens[b] : 0;
-        const int mapped = pages_of(past, a.page_size), fresh = pages_of((long long)past + n, a.page_size) - mapped;
-        long long tokens_before, pages_before;
-        const long long tokens_here = block_scan(n, tokens_before, s_warp);
-        const long long pages_here = block_scan(fresh, pages_before, s_warp);
-        if (b < a.seqs) {
-            past_lens[b] = past;
-            q_starts[b] = (int)(token0 + tokens_before);
-            for (int j = 0; j < fresh; ++j)
-                a.pages[(long long)b * a.max_pages + mapped + j] = a.free_pages[free_count - 1 - (int)(page0 + pages_before) - j];
-            a.lens[b] = past + n;
-        }
-        token0 += tokens_here;
-        page0 += pages_here;
-    }
-    if (tid == 0) {
-        q_starts[a.seqs] = (int)total;
-        *a.free_count = free_count - (int)fresh_total;
-    }
-    __syncthreads();
     // ---- every token's position and slot; rows behind the last token hold -1
-    for (int t = tid; t < max_tokens; t += THREADS) {
-        int position = -1, slot = -1;
-        if (t < total) {
-            int lo = 0, hi = a.seqs;  // the sequence whose [start, next start) holds t
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (q_starts[mid] <= t)
-                    lo = mid;
-                else
-                    hi = mid;
+    const bool aligned = EACH == 4 && (((uintptr_t)positions | (uintptr_t)slots) & 15u) == 0;
+    for (long long t0 = (long long)EACH * i0; t0 < max_tokens; t0 += (long long)EACH * stride) {
+        int position[EACH], slot[EACH];
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) position[j] = slot[j] = -1;
+        if (t0 < total.x) {
+            int b = holder_of(s_start, a.seqs, (int)t0), seen = -1, page = 0;
+            bool lost = false;
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) {
+                if (t0 + j >= total.x) break;
+                if (EACH > 1)
+                    while (t0 + j >= s_start[b + 1]) ++b, seen = -1;
+                const int past = s_past[b], at_token = past + (int)(t0 + j) - s_start[b], at = at_token / a.page_size;
+                if (at != seen) {
+                    const int fresh = at - pages_of(past, a.page_size);
+                    page = fresh >= 0 ? a.free_pages[free_count - 1 - s_fresh[b] - fresh] : a.pages[(long long)b * a.max_pages + at];
+                    seen = at;
+                }
+                const bool there = page >= 0 && page < a.num_pages;
+                lost |= !there;
+                position[j] = at_token;
+                slot[j] = there ? page * a.page_size + at_token - at * a.page_size : -1;
             }
-            position = past_lens[lo] + t - q_starts[lo];
-            const int page = a.pages[(long long)lo * a.max_pages + position / a.page_size];
-            if (page >= 0 && page < a.num_pages)
-                slot = page * a.page_size + position % a.page_size;
-            else
-                atomicOr(a.status, INF_STATUS_BAD_PAGE);
+            if (lost) atomicOr(a.status, INF_STATUS_BAD_PAGE);
         }
-        positions[t] = position;
-        slots[t] = slot;
+        if (aligned && t0 + EACH <= max_tokens) {
+            *reinterpret_cast<int4*>(positions + t0) = make_int4(position[0], position[1 % EACH], position[2 % EACH], position[3 % EACH]);
+            *reinterpret_cast<int4*>(slots + t0) = make_int4(slot[0], slot[1 % EACH], slot[2 % EACH], slot[3 % EACH]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < EACH; ++j)
+                if (t0 + j < max_tokens) positions[t0 + j] = position[j], slots[t0 + j] = slot[j];
+        }
     }
+    // ---- the fresh pages, and the batch's lengths and starts
+    for (int f = i0; f < (int)total.y; f += stride) {
+        const int b = holder_of(s_fresh, a.seqs, f);
+        a.pages[(long long)b * a.max_pages + pages_of(s_past[b], a.page_size) + f - s_fresh[b]] = a.free_pages[free_count - 1 - f];
+    }
+    for (int b = i0; b <= a.seqs; b += stride) {
+        q_starts[b] = s_start[b];
+        if (b < a.seqs) past_lens[b] = s_past[b];
+    }
+    cluster_wait();
+    for (int b = i0; b < a.seqs; b += stride) a.lens[b] = s_past[b] + s_start[b + 1] - s_start[b];
+    if (i0 == 0) *a.free_count = free_count - (int)total.y;
 }
 
 __global__ void __launch_bounds__(THREADS)
 device_index_truncate_kernel(IndexArgs a, const int* __restrict__ keep) {
-    __shared__ long long s_warp[WARPS];
+    __shared__ Sums s_warp[WARPS];
+    extern __shared__ int s_seqs[];
+    int *s_have = s_seqs, *s_hold = s_have + a.seqs, *s_gone = s_hold + a.seqs;  // from the last sequence to the first
     inf_pdl_wait();
     inf_pdl_release();
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, rank = cluster_rank(), i0 = rank * THREADS + tid, stride = (int)gridDim.x * THREADS;
     const int free_count = *a.free_count;
     int bad = free_count < 0 ? INF_STATUS_NO_PAGES : 0;
-    long long gone = 0, unused;
-    for (int b = tid; b < a.seqs; b += THREADS) {
-        const int len = a.lens[b], k = keep[b];
-        if (k >= 0) {
-            if (k > len || len > (long long)a.max_pages * a.page_size)
-                bad |= INF_STATUS_BAD_LEN;
-            else
-                gone += pages_of(len, a.page_size) - pages_of(k, a.page_size);
-        }
+    for (int r = tid; r < a.seqs; r += THREADS) {
+        const int b = a.seqs - 1 - r, len = a.lens[b], k = keep[b];
+        const bool fits = k <= len && len <= (long long)a.max_pages * a.page_size;
+        if (k >= 0 && !fits) bad |= INF_STATUS_BAD_LEN;
+        s_hold[r] = k;
+        s_have[r] = pages_of(len, a.page_size);
+        s_gone[r] = k >= 0 && fits ? s_have[r] - pages_of(k, a.page_size) : 0;
     }
-    const long long gone_total = block_scan(gone, unused, s_warp);
-    if (gone_total + free_count > a.num_pages) bad |= INF_STATUS_NO_PAGES;
-    if (__syncthreads_or(bad)) {
-        if (bad) atomicOr(a.status, bad);
+    const bool any_bad = __syncthreads_or(bad);
+    cluster_arrive();
+    const Sums gone = prefix_sums(s_gone, nullptr, a.seqs, s_warp);
+    const bool overfull = gone.x + free_count > a.num_pages;
+    if (any_bad || overfull) {
+        bad |= overfull ? INF_STATUS_NO_PAGES : 0;
+        if (bad && rank == 0) atomicOr(a.status, bad);
+        cluster_wait();
         return;
     }
-    // from the last sequence to the first, each from its last page down
-    long long pushed0 = 0;
-    for (int r0 = 0; r0 < a.seqs; r0 += THREADS) {
-        const int b = a.seqs - 1 - (r0 + tid);
-        const int len = b >= 0 ? a.lens[b] : 0, k = b >= 0 ? keep[b] : -1;
-        const int have = pages_of(len, a.page_size), hold = k >= 0 ? pages_of(k, a.page_size) : have;
-        long long before;
-        const long long here = block_scan(have - hold, before, s_warp);
-        if (b >= 0 && k >= 0) {
-            for (int j = 0; j < have - hold; ++j) {
-                int* slot = a.pages + (long long)b * a.max_pages + have - 1 - j;
-                a.free_pages[free_count + (int)(pushed0 + before) + j] = *slot;
-                *slot = -1;
-            }
-            a.lens[b] = k;
-        }
-        pushed0 += here;
+    for (int g = i0; g < (int)gone.x; g += stride) {
+        const int r = holder_of(s_gone, a.seqs, g);
+        int* slot = a.pages + (long long)(a.seqs - 1 - r) * a.max_pages + s_have[r] - 1 - (g - s_gone[r]);
+        a.free_pages[free_count + g] = *slot;
+        *slot = -1;
     }
-    if (tid == 0) *a.free_count = free_count + (int)gone_total;
+    cluster_wait();
+    for (int r = i0; r < a.seqs; r += stride)
+        if (s_hold[r] >= 0) a.lens[a.seqs - 1 - r] = s_hold[r];
+    if (i0 == 0) *a.free_count = free_count + (int)gone.x;
+}
+
+// One cluster for `work` threads' work.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), long long work, int seqs, cudaStream_t stream, Args... args) {
+    int ctas = 1;
+    while (ctas < MOST_CTAS && (long long)ctas * THREADS < work) ctas *= 2;
+    const size_t smem = (3 * (size_t)seqs + 2) * sizeof(int);
+    if (smem > 40 * 1024) {  // with the warps' sums more than a launch has without asking
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * MOST_SEQS + 2) * (int)sizeof(int));
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)ctas, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 
 __global__ void device_index_reset_kernel(IndexArgs a) {
@@ -191,6 +275,7 @@ int index_args(inf_ctx* ctx, const inf_device_index* x, const char* what, IndexA
                         x->num_pages, x->page_size, x->max_seqs, x->max_pages);
     if ((long long)x->num_pages * x->page_size > 0x7fffffffLL || (long long)x->max_pages * x->page_size > 0x7fffffffLL)
         return inf_fail(ctx, INF_E_CACHE, "%s: token slots must be countable in 31 bits", what);
+    if (x->max_seqs > MOST_SEQS) return inf_fail(ctx, INF_E_CACHE, "%s: at most %d sequences, got %d", what, MOST_SEQS, x->max_seqs);
     *out = IndexArgs{x->pages, x->lens, x->free_pages, x->free_count, x->num_pages, x->page_size, x->max_seqs, x->max_pages, ctx->status};
     return INF_OK;
 }
@@ -222,7 +307,8 @@ extern "C" int32_t inf_device_index_append(inf_ctx* ctx, const inf_device_index*
         if (!new_tokens || !past_lens || !q_starts || !positions || !slots)
             return inf_fail(ctx, INF_E_ARG, "device_index_append: null pointer");
         if (max_tokens <= 0) return inf_fail(ctx, INF_E_SHAPE, "device_index_append: max_tokens must be positive, got %d", max_tokens);
-        INF_CUDA(ctx, inf_launch_pdl(device_index_append_kernel, dim3(1), dim3(THREADS), 0, ctx->stream, a, new_tokens, max_tokens,
+        const bool few = max_tokens <= MOST_CTAS * THREADS;
+        INF_CUDA(ctx, launch_cluster(few ? device_index_append_kernel<1> : device_index_append_kernel<4>, max_tokens, a.seqs, ctx->stream, a, new_tokens, max_tokens,
                                      past_lens, q_starts, positions, slots));
         return INF_OK;
     });
@@ -235,7 +321,8 @@ extern "C" int32_t inf_device_index_truncate(inf_ctx* ctx, const inf_device_inde
         const int rc = index_args(ctx, index, "device_index_truncate", &a);
         if (rc != INF_OK) return rc;
         if (!keep_lens) return inf_fail(ctx, INF_E_ARG, "device_index_truncate: null pointer");
-        INF_CUDA(ctx, inf_launch_pdl(device_index_truncate_kernel, dim3(1), dim3(THREADS), 0, ctx->stream, a, keep_lens));
+        // how many pages go is known on the GPU alone: four a sequence are expected
+        INF_CUDA(ctx, launch_cluster(device_index_truncate_kernel, 4LL * a.seqs, a.seqs, ctx->stream, a, keep_lens));
         return INF_OK;
     });
 }

@@ -25,7 +25,7 @@ def ints(be, v):
 
 
 # ------------------------------------------------------------------------------------------------ index
-@pytest.mark.parametrize("seqs,P,max_tokens", [(1, 16, 40), (7, 16, 900), (33, 48, 300), (1500, 1, 5000), (2100, 64, 70000)])
+@pytest.mark.parametrize("seqs,P,max_tokens", [(1, 16, 40), (7, 16, 900), (33, 48, 300), (1500, 1, 5000), (2100, 64, 70000), (16384, 16, 60000)])
 def test_device_index_follows_the_host_index(be, seqs, P, max_tokens):
     """A random run of appends and cuts: table, lengths, order of the free list as the host's one-by-one bookkeeping."""
     from inferno_b200.paged import PagedIndex
@@ -94,6 +94,24 @@ def test_append_then_truncate_restores_the_index(be):
     be.device_flush()
     for was, t in zip(before, (index.pages, index.lens, index.free_pages, index.free_count)):
         assert torch.equal(was, t)
+
+
+@pytest.mark.parametrize("max_tokens", [50, 20001])
+def test_index_outputs_at_any_word(be, max_tokens):
+    """Layout buffers that start between 16-byte boundaries, as views of a larger one do; words around them stay."""
+    index = be.prepare_device_index(3000, 16, 5, 2000)
+    want = be.device_index_append(index, ints(be, [7, 0, max_tokens // 2, 3, 1]), be.prepare_ragged_batch(5, max_tokens))
+    be.device_index_truncate(index, want.past_lens)
+    arena = torch.full((2 * max_tokens + 64,), -7, dtype=torch.int32, device=be.device)
+    sizes, at, views = (5, 6, max_tokens, max_tokens), 1, []
+    for n in sizes:
+        views.append(arena[at:at + n])
+        at += n + 2
+    got = be.device_index_append(index, ints(be, [7, 0, max_tokens // 2, 3, 1]), type(want)(*views))
+    be.device_flush()
+    for name in ("past_lens", "q_starts", "positions", "slots"):
+        assert torch.equal(getattr(got, name), getattr(want, name)), name
+    assert int((arena == -7).sum()) == arena.numel() - sum(sizes)
 
 
 @pytest.mark.parametrize("new,max_tokens,why", [
@@ -439,6 +457,7 @@ def test_refusals(be):
     refuses("ShapeMismatch", app, q, k, k, rope, pool, pos, slots, q_norm=torch.ones(64, device=be.device))
     refuses("Argument", app, q, k, torch.randn((2, 5, 128), device=be.device).transpose(0, 1), rope, pool, pos, slots)
     refuses("Argument", app, torch.randn((5, 12 * 128 + 2), device=be.device)[:, :12 * 128].unflatten(1, (12, 128)), k, k, rope, pool, pos, slots)
+    refuses("Argument", app, q, k, k, rope, pool, pos, slots, k_norm=torch.ones(129, device=be.device)[1:])
     refuses("Config", app, q, k, k, None, pool, pos, slots, q_norm=torch.ones(128, device=be.device))
     refuses("Config", app, q, k, k, rope, pool, pos, slots, eps=float("nan"))
     assert app(q[:0], k[:0], k[:0], rope, pool, pos[:0], slots[:0]).shape == (0, 12, 128)
@@ -450,6 +469,7 @@ def test_refusals(be):
     assert torch.equal(pool.v[0, :, 4], k[4].half()) and (pool.v[0, :, 1] == 0).all()
 
     refuses("Cache", be.prepare_device_index, 0, 16, 1, 1)
+    refuses("Cache", be.prepare_device_index, 8, 16, 16385, 1)
     index = be.prepare_device_index(8, 16, 2, 4)
     refuses("ShapeMismatch", be.prepare_ragged_batch, 2, 0)
     batch = be.prepare_ragged_batch(2, 10)
