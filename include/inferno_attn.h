@@ -503,11 +503,13 @@ int32_t inf_rope_append_gqa_ragged(inf_ctx* ctx, const void* q, const void* k, c
  * them, and their own keys and values have been appended at lens[b] onwards.  Row t sees keys [max(0, p + 1 - window), p],
  * p = lens[b] + t.  gate f32 [tokens][q_heads] (optional) applies softplus(gate); scale <= 0 means 1/sqrt(128); out
  * [tokens][q_heads][128] in out_dtype.  Rows from q_starts[batch] on are left as they were.  Up to 128 query heads per KV
- * head (INF_UNSUPPORTED beyond) and 2^29 tokens in a row of the page table.  A sequence whose rows or length do not fit is skipped and reported, a page id outside
- * the pool is reported and its keys read as zeros.  Keys and values of a sequence's tokens must be finite; pool slots behind
- * its last token may hold anything.  The context's first call allocates scratch (about 40 MB); make it before a capture.
- * Calls of one context, and graphs captured through it, share that scratch and must not overlap on the GPU: work that runs
- * at the same time takes a context each. */
+ * head (INF_UNSUPPORTED beyond) and 2^29 tokens in a row of the page table.  A sequence whose rows or length do not fit is
+ * skipped and reported, a page id outside the pool is reported and its keys read as zeros.  Keys and values that some row of
+ * the call sees must be finite: one that is not may reach other rows of its sequence.  Pool slots that no row sees, behind a
+ * sequence's last token and below its first row's window, may hold anything; pages wholly below that window may have been
+ * given back.  The context's first call allocates scratch (about 40 MB); make it before a capture.  Calls of one context, and
+ * graphs captured through it, share that scratch and must not overlap on the GPU: work that runs at the same time takes a
+ * context each. */
 int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, const inf_kv_pool* pool, const inf_page_table* table,
                                  const int32_t* q_starts, int32_t tokens, int32_t q_heads, int32_t sliding_window,
                                  const float* gate, float scale, void* out, int32_t out_dtype);

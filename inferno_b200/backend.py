@@ -253,13 +253,18 @@ class CudaBackend:
         self._check(self._lib.inf_download(self._ctx, C.c_void_p(out.data_ptr()), _ptr(dev), dev.numel() * 4))
         return out
 
+    def _here(self, what: str, *tensors):
+        """The tensors behind a descriptor: on this context's GPU."""
+        for t in tensors:
+            if t.device != self.device:
+                raise InfernoError(L.INF_E_ARG, f"{what}: tensor on {t.device}, the context is on {self.device}")
+
     def _mine(self, what: str, dtype, *tensors, contiguous: bool = True):
         """The arguments of one call: on this context's GPU, of one dtype, contiguous unless the call takes strides."""
         for t in tensors:
             if t is None:
                 continue
-            if t.device != self.device:
-                raise InfernoError(L.INF_E_ARG, f"{what}: tensor on {t.device}, the context is on {self.device}")
+            self._here(what, t)
             if t.dtype != dtype:
                 raise InfernoError(L.INF_E_DTYPE, f"{what}: expected {dtype}, got {t.dtype}")
             if contiguous and not t.is_contiguous():
@@ -268,7 +273,7 @@ class CudaBackend:
     def _new(self, shape, dtype) -> torch.Tensor:
         """Memory for an output that the library's stream writes: from that stream's pool, so that no other stream's
         pending work still uses it."""
-        if self.stream.cuda_stream == torch.cuda.current_stream(self.device).cuda_stream:
+        if self.stream.cuda_stream == torch.cuda.current_stream(self.device.index).cuda_stream:
             return torch.empty(shape, dtype=dtype, device=self.device)
         with torch.cuda.stream(self.stream):
             return torch.empty(shape, dtype=dtype, device=self.device)
@@ -368,6 +373,7 @@ class CudaBackend:
     def device_index_append(self, index: DeviceIndex, new_tokens: torch.Tensor, batch: RaggedBatch) -> RaggedBatch:
         """Reserve new_tokens[b] more slots per sequence; the step's layout goes into `batch`.  A step that does not fit
         changes nothing, describes no tokens and is reported by device_flush."""
+        self._here("device_index_append", index.pages)
         self._mine("device_index_append", torch.int32, new_tokens, batch.past_lens, batch.q_starts, batch.positions, batch.slots)
         seqs = index.desc.max_seqs
         if new_tokens.shape != (seqs,) or batch.past_lens.shape != (seqs,) or batch.q_starts.shape != (seqs + 1,) \
@@ -380,6 +386,7 @@ class CudaBackend:
 
     def device_index_truncate(self, index: DeviceIndex, keep_lens: torch.Tensor):
         """Cut sequence b to keep_lens[b] tokens (0 releases it, negative leaves it alone); its pages become free."""
+        self._here("device_index_truncate", index.pages)
         self._mine("device_index_truncate", torch.int32, keep_lens)
         if keep_lens.shape != (index.desc.max_seqs,):
             raise InfernoError(L.INF_E_SHAPE, f"device_index_truncate: the index has {index.desc.max_seqs} sequences, got {tuple(keep_lens.shape)} lengths")
@@ -393,6 +400,7 @@ class CudaBackend:
         if q.dtype not in (torch.float32, torch.float16):
             raise InfernoError(L.INF_E_DTYPE, "rope_append_gqa_ragged: q/k/v must share dtype f32 or f16")
         what, d, hkv = "rope_append_gqa_ragged", pool.desc.head_dim, pool.desc.kv_heads
+        self._here(what, pool.k)
         self._mine(what, q.dtype, q, k, v, contiguous=False)
         self._mine(what, torch.int32, positions, slots)
         self._mine(what, torch.float32, q_norm, k_norm)
@@ -426,6 +434,7 @@ class CudaBackend:
         belong to sequence b, table.lens counts the keys cached before them.  Rows behind the last sequence's keep
         what `out` holds."""
         what = "gqa_attention_ragged"
+        self._here(what, pool.k, table.pages)
         self._mine(what, torch.float16, q_f16)
         self._mine(what, torch.int32, q_starts)
         self._mine(what, torch.float32, gate)

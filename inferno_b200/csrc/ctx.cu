@@ -190,6 +190,9 @@ int32_t inf_flush(inf_ctx* ctx) {
     int s = ctx->host_status[0];
     if (s != 0) {
         INF_CUDA(ctx, cudaMemsetAsync(ctx->status, 0, 16, ctx->stream));
+        // a ragged attention that gave up may have left pieces uncounted
+        if ((s & INF_STATUS_WAIT_TIMEOUT) && ctx->ragged_counters)
+            INF_CUDA(ctx, cudaMemsetAsync(ctx->ragged_counters, 0, ctx->sm_count * sizeof(int), ctx->stream));
         return inf_fail(ctx, INF_E_BACKEND, "device status word 0x%x:%s%s%s%s%s", s,
                         (s & INF_STATUS_WAIT_TIMEOUT) ? " bounded wait gave up;" : "",
                         (s & INF_STATUS_BAD_PAGE) ? " page id outside the pool;" : "",

@@ -281,6 +281,11 @@ __device__ __forceinline__ int dead_slots(const RaggedParams& p, const Item& it,
     return live < BN ? (live + p.box_rows - 1) / p.box_rows * p.box_rows - live : 0;
 }
 
+// Slots of key tile t below the lowest key any row sees, in the box that brings that key.
+__device__ __forceinline__ int dead_below(const RaggedParams& p, const Item& it, int t) {
+    return it.lowest > t * BN ? (it.lowest - t * BN) % p.box_rows : 0;
+}
+
 // Who reads a tile last: (stream, that stream's count of tiles) of the last three tiles, so that a producer knows which
 // barrier says that a ring slot is free.  MMAs of one thread retire in order, so the last reader speaks for both.
 struct TileLog {
@@ -756,13 +761,17 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     }
                     walk.load(&tm_v, p, t, sV + (tiles % VS) * TILE_BYTES, &sh.v_full[tiles % VS]);
                     log.add(shared_rows, (t - it.kt0) & 1);
-                    // slots of the last box behind the sequence's last key may hold anything, and 0 * NaN is NaN
-                    const int dead = dead_slots(p, it, t);
-                    if (dead) {
+                    // slots that no row sees may hold anything, and 0 * NaN is NaN
+                    const int behind = dead_slots(p, it, t), below = dead_below(p, it, t);
+                    if (behind | below) {
                         alive = warp_wait(&sh.v_full[tiles % VS], (uint32_t)(tiles / VS) & 1u);
-                        uint8_t* at = sV + (tiles % VS) * TILE_BYTES + (it.kv_total - t * BN) * 128;
-                        for (int c = lane; c < dead * 16; c += 32)
-                            *reinterpret_cast<uint4*>(at + ((c >> 3) & 1) * BLK_BYTES + (c >> 4) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        auto clear = [&](int row, int rows) {
+                            uint8_t* at = sV + (tiles % VS) * TILE_BYTES + row * 128;
+                            for (int c = lane; c < rows * 16; c += 32)
+                                *reinterpret_cast<uint4*>(at + ((c >> 3) & 1) * BLK_BYTES + (c >> 4) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        };
+                        clear(it.kv_total - t * BN, behind);
+                        clear(it.lowest - t * BN - below, below);
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sh.v_patched[tiles % VS]);
@@ -821,6 +830,10 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                                     &sh.q_full[1]);
                 }
             }
+            if (!alive) {  // copies in flight land before the block ends
+                if (uses0 > 0) warp_wait(&sh.q_full[0], (uint32_t)(uses0 - 1) & 1u);
+                if (uses1 > 0) warp_wait(&sh.q_full[1], (uint32_t)(uses1 - 1) & 1u);
+            }
         } else {
             // ------------------------------------------------ every MMA, from one thread.  It runs about four MMAs (256
             // cycles) ahead of the tensor cores; what it does between two groups must not take longer, so ring positions and
@@ -836,7 +849,9 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             while (lane == 0 && (alive = reader.next_for_one_thread(sh, it)) && it.kt0 < it.kt1) {
                 const bool shared_rows = shares_rows(p, it);
                 const int steps = (it.kt1 - it.kt0) * (shared_rows ? 1 : 2);  // one tile of one stream each, the streams in turn
+                // steps whose V tile is cleared first: the one of the item's last key, the one of its lowest
                 const int dead_step = dead_slots(p, it, it.kt1 - 1) ? (shared_rows ? steps - 1 : steps - 2) : -1;
+                const int low_step = dead_below(p, it, it.kt0) ? 0 : -1;
                 uint32_t k_lo = 0, v_lo = 0;
                 alive = lone_wait(&sh.q_full[0], q_parity & 1u);
                 q_parity ^= 1u;
@@ -853,7 +868,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     if (w >= 2) {
                         if (new_tile) {
                             alive = alive && lone_wait(&sh.v_full[v_at.slot], v_at.parity);
-                            if (w - 2 == dead_step) {
+                            if (w - 2 == dead_step || w - 2 == low_step) {
                                 alive = alive && lone_wait(&sh.v_patched[v_at.slot], (patched >> v_at.slot) & 1u);
                                 patched ^= 1u << v_at.slot;
                             }
@@ -1090,16 +1105,18 @@ int ragged_scratch(inf_ctx* ctx, int grid, float** acc, float** ml, int** counte
     if (!ctx->ragged_scratch) {
         void* fresh = nullptr;
         INF_CUDA(ctx, cudaMalloc(&fresh, bytes));
-        const cudaError_t e = cudaMemsetAsync(fresh, 0, bytes, ctx->stream);
+        cudaError_t e = cudaMemsetAsync(fresh, 0, bytes, ctx->stream);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);  // the next call may be on another stream
         if (e != cudaSuccess) {
             cudaFree(fresh);
             return inf_fail(ctx, INF_E_BACKEND, "gqa_attention_ragged: clearing the scratch failed: %s", cudaGetErrorString(e));
         }
         ctx->ragged_scratch = fresh;
+        ctx->ragged_counters = (int*)((float*)fresh + rows * (D + 2));
     }
     *acc = (float*)ctx->ragged_scratch;
     *ml = *acc + rows * D;
-    *counters = (int*)(*ml + rows * 2);
+    *counters = ctx->ragged_counters;
     return INF_OK;
 }
 
@@ -1126,7 +1143,7 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
             return inf_fail(ctx, INF_E_SHAPE, "%s: q_heads %d must be a positive multiple of kv_heads %d", what, q_heads, pool->kv_heads);
         if (q_heads / pool->kv_heads > 128) return INF_UNSUPPORTED;
         if (sliding_window < 0) return inf_fail(ctx, INF_E_CONFIG, "%s: sliding_window must be >= 0", what);
-        if (!isfinite(scale)) return inf_fail(ctx, INF_E_CONFIG, "%s: scale must be finite", what);
+        if (!(scale <= 1e15f)) return inf_fail(ctx, INF_E_CONFIG, "%s: scale must be finite and at most 1e15", what);
         if (out_dtype != INF_DTYPE_F32 && out_dtype != INF_DTYPE_F16)
             return inf_fail(ctx, INF_E_DTYPE, "%s: output dtype must be f32 or f16", what);
         int rc = inf_validate_table(ctx, table, pool->num_pages, pool->page_size, 0, what, sliding_window, 1);

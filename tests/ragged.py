@@ -73,7 +73,7 @@ def assert_attention_close(got, want, size, keys, what=""):
 
 
 class Batch:
-    """Pools with cached and new tokens of several sequences in scattered pages; slots that hold no token hold `filler`."""
+    """Pools with cached and new tokens of several sequences in scattered pages; slots that no new token sees hold `filler`."""
 
     def __init__(self, device, past, new, Hq, Hkv, P=16, seed=0, filler=float("nan"), window=0, spare_rows=0, tight=True):
         g = torch.Generator(device=device).manual_seed(seed)
@@ -93,6 +93,8 @@ class Batch:
             for pool in (self.k, self.v):
                 rows = torch.randn((c * P, Hkv, 128), generator=g, device=device, dtype=torch.float16)
                 rows[total:] = filler
+                if window:
+                    rows[:max(0, past[b] + 1 - window)] = filler  # below every new row's window
                 pool[self.pages[b, :c].long()] = rows.view(c, P, Hkv, 128).transpose(1, 2)
         starts = [0]
         for n in new:

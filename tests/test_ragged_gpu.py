@@ -262,6 +262,42 @@ def test_attention_ragged_twice_gives_the_same_bits(be):
     assert torch.equal(b.check(be), b.check(be))
 
 
+@pytest.mark.parametrize("past,new,Hq,Hkv", [
+    ([30000, 7], [2, 90], 12, 2),  # one item cut many times, a light one; two streams
+    ([9000], [130], 12, 2),
+    ([30000], [5], 64, 8),
+    ([100, 3], [20, 1], 12, 2),
+])
+def test_attention_ragged_keeps_nothing_of_the_call_before(be, past, new, Hq, Hkv):
+    """Tiles, TMEM and scratch full of NaN from another call leave every bit of the next one alone."""
+    b = Batch(be.device, past, new, Hq, Hkv, 16, seed=20)
+    d = Batch(be.device, past, new, Hq, Hkv, 16, seed=20)
+    d.q.fill_(float("nan"))
+
+    def run(x):
+        return be.gqa_attention_ragged(x.q, be.kv_pool(x.k, x.v), be.page_table(x.pages, x.past_lens, validate_on_host=False),
+                                       x.q_starts, out_dtype=torch.float32)
+
+    first = run(b)
+    assert torch.isnan(run(d)).all()
+    assert torch.equal(run(b), first)
+    be.device_flush()
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
+def test_attention_ragged_rows_at_odd_sixteen_bytes(be, out_dtype):
+    """Queries and output that begin 16 bytes into a 32-byte sector."""
+    b = Batch(be.device, [300, 5000, 40], [90, 2, 30], 12, 2, 16, seed=21)
+    pool, table = be.kv_pool(b.k, b.v), be.page_table(b.pages, b.past_lens, validate_on_host=False)
+    want = be.gqa_attention_ragged(b.q, pool, table, b.q_starts, out_dtype=out_dtype)
+    pad = 8 if out_dtype == torch.float16 else 4
+    q = torch.empty(b.q.numel() + 8, dtype=torch.float16, device=be.device)[8:].view(b.q.shape).copy_(b.q)
+    arena = torch.full((b.q.numel() + 2 * pad,), 7.0, dtype=out_dtype, device=be.device)
+    got = be.gqa_attention_ragged(q, pool, table, b.q_starts, out=arena[pad:-pad].view(b.q.shape))
+    be.device_flush()
+    assert torch.equal(got, want) and (arena[:pad] == 7).all() and (arena[-pad:] == 7).all()
+
+
 def test_attention_ragged_large_and_equal_scores(be):
     """Scores in the hundreds (the softmax is one key), and equal ones (the mean of the values)."""
     b = Batch(be.device, [300], [60], 12, 2, 16, seed=4, filler=0.0)
@@ -436,7 +472,8 @@ def test_refusals(be):
     refuses("ShapeMismatch", att, b.q, pool, table, b.q_starts, gate=b.gate[:2].contiguous())
     refuses("ShapeMismatch", att, b.q, pool, table, b.q_starts, out=torch.empty_like(b.q[:2]))
     refuses("Config", att, b.q, pool, table, b.q_starts, sliding_window=-1)
-    refuses("Config", att, b.q, pool, table, b.q_starts, scale=float("nan"))
+    for scale in (float("nan"), float("inf"), 1e16):
+        refuses("Config", att, b.q, pool, table, b.q_starts, scale=scale)
     refuses("Argument", att, b.q.transpose(0, 1), pool, table, b.q_starts)
     refuses("Argument", att, b.q.cpu(), pool, table, b.q_starts)
     assert att(torch.zeros((4, 258, 128), dtype=torch.float16, device=be.device), pool, table, b.q_starts) is None  # 129 heads per KV head
