@@ -30,7 +30,9 @@
 //
 // Rows of few items fill few of the 128 lanes, and a warp's exponentials go through one of the four special-function
 // units.  Up to 32 rows (decodes, short drafts) are therefore dealt out to the four lane quarters, and each is held by four
-// threads (16x256 TMEM shape): 32 exponentials a thread and tile instead of 128 on one warp.
+// threads (16x256 TMEM shape): 32 exponentials a thread and tile instead of 128 on one warp.  Their MMAs are of M64, whose
+// rows are lanes 0-15 of each quarter: a batch of decodes holds the GPU at its power limit, and half the multiplications
+// leave the clock 8 % higher (139 -> 133 us).
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -250,6 +252,35 @@ __device__ __forceinline__ bool lone_wait(uint64_t* bar, uint32_t parity) {
 // of a whole warp, with one answer for all its lanes
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, lone_wait(bar, parity)); }
 
+// of a whole warp without a vote, so that its branches stay uniform: a wait that gave up leaves the ones after it no tries
+__device__ __forceinline__ void uniform_wait(uint64_t* bar, uint32_t parity, uint32_t& tries) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 tried;\n\t"
+        "mov.u32 tried, 0;\n"
+        "again:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "add.u32 tried, tried, 1;\n\t"
+        "setp.lt.u32 q, tried, %3;\n\t"
+        "@p bra done;\n\t"
+        "@q bra again;\n"
+        "done:\n\t"
+        "selp.u32 %0, %3, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(tries)
+        : "memory");
+    tries = ok;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t leader;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(leader));
+    return leader != 0;
+}
+
 // A role's view of the items: the next one's description, copied to registers.
 struct ItemReader {
     int count = 0;
@@ -259,14 +290,6 @@ struct ItemReader {
         it = sh.items[slot];
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.item_free[slot]);
-        ++count;
-        return true;
-    }
-    __device__ __forceinline__ bool next_for_one_thread(Shared& sh, Item& it) {  // the warp's other lanes have left
-        const int slot = count % RING;
-        if (!lone_wait(&sh.item_full[slot], (uint32_t)(count / RING) & 1u)) return false;
-        it = sh.items[slot];
-        mbar_arrive(&sh.item_free[slot]);
         ++count;
         return true;
     }
@@ -606,8 +629,8 @@ __device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& i
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
-ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                        const __grid_constant__ CUtensorMap tm_v, RaggedParams p) {
+ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_q_light,
+                        const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, RaggedParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *sQ = smem, *sK = smem + OFF_K, *sV = smem + OFF_V;
     Shared& sh = *reinterpret_cast<Shared*>(smem + OFF_SHARED);
@@ -643,9 +666,12 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     }
     if (warp == 8 && lane == 0) {
         tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_q_light);
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
     }
+    for (int i = tid; i < TILE_BYTES / 16; i += THREADS) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
     inf_pdl_wait();  // queries, appended rows, lengths and page table come from work earlier in the stream
     inf_pdl_release();
     const bool has_work = find_part(p, sh) && smem_ok;
@@ -783,28 +809,42 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             if (!alive)
                 for (int t = max(0, tiles - VS); t < tiles; ++t) warp_wait(&sh.v_full[t % VS], (uint32_t)(t / VS) & 1u);
         } else if (warp == 11) {
-            // ------------------------------------------------ Q: a stream's tile is free when its last S has retired
+            // ------------------------------------------------ Q: a stream's tile is free when its last S has retired.  An item of
+            // few or light rows finds zeros in the tile's other rows: the tensor cores work on all 128, and what they draw for
+            // multiplying by zero leaves the clock higher when the GPU is at its power limit.
             int uses0 = 0, uses1 = 0;
+            int held = 0;  // rows of stream 0's tile that are not zero: of an item of few rows, or -1: light, -2: any
+            auto few_row = [](int r) { return (r & 3) * 16 + (r >> 2); };  // row r of few lies there
+            auto zero_chunk = [&](int row, int chunk) {
+                *reinterpret_cast<uint4*>(sQ + (chunk >> 3) * BLK_BYTES + row * 128 + ((chunk & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            };
             while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
                 if (uses0 > 0) alive = warp_wait(&sh.q_free[0], (uint32_t)(uses0 - 1) & 1u);
                 if (!alive) break;
                 ++uses0;
+                const int rows = it.ntok * p.group;
                 if (few_rows(p, it)) {
-                    // row r to lane (r % 4) * 32 + r / 4, with the swizzle that a TMA load would have written
-                    const int chunks = it.ntok * p.group * 16;
-                    for (int c0 = 0; c0 < chunks; c0 += 4 * 32) {
+                    // as a TMA load with the swizzle would have written them
+                    if (held < 0) {
+                        for (int c = lane; c < BM * 16; c += 32) zero_chunk(c >> 4, c & 15);
+                        __syncwarp();
+                    } else {
+                        for (int c = rows * 16 + lane; c < held * 16; c += 32) zero_chunk(few_row(c >> 4), c & 15);
+                    }
+                    held = rows;
+                    for (int c0 = 0; c0 < rows * 16; c0 += 4 * 32) {
                         uint4 v[4];
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
                             const int c = c0 + u * 32 + lane, r = c >> 4;
-                            if (c < chunks)
+                            if (r < rows)
                                 v[u] = *reinterpret_cast<const uint4*>(
                                     p.q + ((long long)(it.tok0 + r / p.group) * p.q_heads + it.kvh * p.group + r % p.group) * D + (c & 15) * 8);
                         }
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
-                            const int c = c0 + u * 32 + lane, r = c >> 4, row = (r & 3) * 32 + (r >> 2);
-                            if (c < chunks)
+                            const int c = c0 + u * 32 + lane, r = c >> 4, row = few_row(r);
+                            if (r < rows)
                                 *reinterpret_cast<uint4*>(sQ + ((c >> 3) & 1) * BLK_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[u];
                         }
                     }
@@ -813,11 +853,18 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     if (lane == 0) mbar_arrive(&sh.q_full[0]);
                     continue;
                 }
+                const bool light = it.ntok <= p.light_tokens;
+                if (light && held != -1) {
+                    for (int c = LIGHT_ROWS * 16 + lane; c < BM * 16; c += 32) zero_chunk(c >> 4, c & 15);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                held = light ? -1 : -2;
                 const uint32_t bytes = (uint32_t)(p.stream_tokens * p.group) * 256u;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&sh.q_full[0], bytes);
+                    mbar_arrive_expect_tx(&sh.q_full[0], light ? (uint32_t)(p.light_tokens * p.group) * 256u : bytes);
                     for (int blk = 0; blk < 2; ++blk)
-                        tma_load_3d(sQ + blk * BLK_BYTES, &tm_q, blk * 64, it.kvh * p.group, it.tok0, &sh.q_full[0]);
+                        tma_load_3d(sQ + blk * BLK_BYTES, light ? &tm_q_light : &tm_q, blk * 64, it.kvh * p.group, it.tok0, &sh.q_full[0]);
                 }
                 if (shares_rows(p, it)) continue;
                 if (uses1 > 0) alive = warp_wait(&sh.q_free[1], (uint32_t)(uses1 - 1) & 1u);
@@ -835,10 +882,12 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 if (uses1 > 0) warp_wait(&sh.q_full[1], (uint32_t)(uses1 - 1) & 1u);
             }
         } else {
-            // ------------------------------------------------ every MMA, from one thread.  It runs about four MMAs (256
-            // cycles) ahead of the tensor cores; what it does between two groups must not take longer, so ring positions and
-            // parities are stepped, not computed, and the loop is short.
-            constexpr uint32_t idesc_s = umma_idesc_f16(BM, BN, 0, 0), idesc_o = umma_idesc_f16(BM, D, 0, 1);
+            // ------------------------------------------------ every MMA.  The warp runs about four MMAs (256 cycles) ahead of the
+            // tensor cores; what it does between two groups must not take longer.  So its branches depend on values that are the
+            // same in all lanes, which keeps descriptors and addresses in uniform registers (as a lone thread's, moved there for
+            // each MMA, the chunk of 4096 took 5 % longer), and ring positions and parities are stepped, not computed.
+            constexpr uint32_t idesc_s128 = umma_idesc_f16(BM, BN, 0, 0), idesc_o128 = umma_idesc_f16(BM, D, 0, 1),
+                               idesc_s64 = umma_idesc_f16(BM / 2, BN, 0, 0), idesc_o64 = umma_idesc_f16(BM / 2, D, 0, 1);
             constexpr uint32_t hi = umma_desc_hi(1024, UMMA_SW128);
             const uint32_t q_lo0 = umma_desc_lo(smem_u32(sQ), 16), k_lo0 = umma_desc_lo(smem_u32(sK), 16),
                            v_lo0 = umma_desc_lo(smem_u32(sV), BLK_BYTES);
@@ -846,30 +895,34 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             RingPlace<VS> v_at;
             RingPlace<SR> s_at[2], o_at[2];  // which barriers the next S and PV of a stream report to
             uint32_t patched = 0, p_parity = 0, q_parity = 0;  // a bit for each V slot, stream, stream
-            while (lane == 0 && (alive = reader.next_for_one_thread(sh, it)) && it.kt0 < it.kt1) {
-                const bool shared_rows = shares_rows(p, it);
-                const int steps = (it.kt1 - it.kt0) * (shared_rows ? 1 : 2);  // one tile of one stream each, the streams in turn
+            const uint32_t tb = __shfl_sync(0xffffffffu, tbase, 0);
+            uint32_t tries = 0x200000u;  // none once a wait gave up
+            while ((alive = reader.next(sh, it)) && it.kt0 < it.kt1) {
+                const bool shared_rows = __shfl_sync(0xffffffffu, shares_rows(p, it) ? 1 : 0, 0) != 0;
+                const uint32_t few = __shfl_sync(0xffffffffu, few_rows(p, it) ? 1u : 0u, 0);
+                const uint32_t idesc_s = few ? idesc_s64 : idesc_s128, idesc_o = few ? idesc_o64 : idesc_o128;
+                const int steps = __shfl_sync(0xffffffffu, (it.kt1 - it.kt0) * (shared_rows ? 1 : 2), 0);  // one tile of one stream each, the streams in turn
                 // steps whose V tile is cleared first: the one of the item's last key, the one of its lowest
-                const int dead_step = dead_slots(p, it, it.kt1 - 1) ? (shared_rows ? steps - 1 : steps - 2) : -1;
-                const int low_step = dead_below(p, it, it.kt0) ? 0 : -1;
+                const int dead_step = __shfl_sync(0xffffffffu, dead_slots(p, it, it.kt1 - 1) ? (shared_rows ? steps - 1 : steps - 2) : -1, 0);
+                const int low_step = __shfl_sync(0xffffffffu, dead_below(p, it, it.kt0) ? 0 : -1, 0);
                 uint32_t k_lo = 0, v_lo = 0;
-                alive = lone_wait(&sh.q_full[0], q_parity & 1u);
+                uniform_wait(&sh.q_full[0], q_parity & 1u, tries);
                 q_parity ^= 1u;
                 if (!shared_rows) {
-                    alive = alive && lone_wait(&sh.q_full[1], q_parity >> 1);
+                    uniform_wait(&sh.q_full[1], q_parity >> 1, tries);
                     q_parity ^= 2u;
                 }
                 // step w: PV of tile w - 2 of the steps, then S of tile w
 #pragma unroll 1
                 for (int w = 0; w < steps + 2; ++w) {
                     const int st = w & 1;
-                    const uint32_t col_s = tbase + COL_S + st * BN, col_o = tbase + COL_O + st * D;
+                    const uint32_t col_s = tb + COL_S + st * BN, col_o = tb + COL_O + st * D;
                     const bool new_tile = shared_rows || st == 0;
                     if (w >= 2) {
                         if (new_tile) {
-                            alive = alive && lone_wait(&sh.v_full[v_at.slot], v_at.parity);
+                            uniform_wait(&sh.v_full[v_at.slot], v_at.parity, tries);
                             if (w - 2 == dead_step || w - 2 == low_step) {
-                                alive = alive && lone_wait(&sh.v_patched[v_at.slot], (patched >> v_at.slot) & 1u);
+                                uniform_wait(&sh.v_patched[v_at.slot], (patched >> v_at.slot) & 1u, tries);
                                 patched ^= 1u << v_at.slot;
                             }
                             v_lo = v_lo0 + v_at.slot * (TILE_BYTES >> 4);
@@ -877,17 +930,19 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                         }
 #pragma unroll 1
                         for (int half = 0; half < 2; ++half) {  // the halves of P arrive separately
-                            alive = alive && lone_wait(&sh.p_full[st][half], (p_parity >> st) & 1u);
-                            if (!alive) break;
+                            uniform_wait(&sh.p_full[st][half], (p_parity >> st) & 1u, tries);
                             tc_fence_after();
+                            if (elect_one()) {
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)
-                                umma_ts(col_o, col_s + half * 32 + kk * 8, umma_desc_pack(v_lo + (half * 4 + kk) * (2048 >> 4), hi), idesc_o,
-                                        kk > 0 || half > 0 || w >= 4);
+                                for (int kk = 0; kk < 4; ++kk)
+                                    umma_ts(col_o, col_s + half * 32 + kk * 8, umma_desc_pack(v_lo + (half * 4 + kk) * (2048 >> 4), hi), idesc_o,
+                                            kk > 0 || half > 0 || w >= 4);
+                            }
+                            __syncwarp();
                         }
-                        if (!alive) break;
                         p_parity ^= 1u << st;
-                        tc_commit(&sh.o_ready[st][st ? o_at[1].slot : o_at[0].slot]);
+                        if (elect_one()) tc_commit(&sh.o_ready[st][st ? o_at[1].slot : o_at[0].slot]);
+                        __syncwarp();
                         if (st)
                             o_at[1].step();
                         else
@@ -895,25 +950,28 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     }
                     if (w < steps) {
                         if (new_tile) {
-                            alive = alive && lone_wait(&sh.k_full[k_at.slot], k_at.parity);
+                            uniform_wait(&sh.k_full[k_at.slot], k_at.parity, tries);
                             k_lo = k_lo0 + k_at.slot * (TILE_BYTES >> 4);
                             k_at.step();
                         }
-                        if (!alive) break;
                         const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
+                        if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
-                            umma_ss(col_s, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
+                            for (int kk = 0; kk < 8; ++kk) {
+                                const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
+                                umma_ss(col_s, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
+                            }
+                            tc_commit(&sh.s_full[st][st ? s_at[1].slot : s_at[0].slot]);
+                            if (w + 1 == steps || (!shared_rows && w + 2 == steps)) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
                         }
-                        tc_commit(&sh.s_full[st][st ? s_at[1].slot : s_at[0].slot]);
+                        __syncwarp();
                         if (st)
                             s_at[1].step();
                         else
                             s_at[0].step();
-                        if (w + 1 == steps || (!shared_rows && w + 2 == steps)) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
                     }
                 }
+                alive = __all_sync(0xffffffffu, tries != 0);
                 if (!alive) break;
             }
         }
@@ -941,7 +999,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             const int row_tok = r / p.group;
             const int qpos_lo = it.qpos0 + tok_in, qpos_hi = qpos_lo + (rows - 1) / p.group;  // of the stream's rows
             const int qpos = qpos_lo + row_tok, first_key = p.window > 0 ? qpos + 1 - p.window : 0;
-            float m_used = M_INIT, l = 0.f;
+            float m_used = valid ? M_INIT : -M_INIT, l = 0.f;  // no row there: its weights are zeros
             for (int j = 0; j < n; ++j, ++cnt) {
                 const int k0 = (first_tile + j * step) * BN;
                 if (ok) ok = warp_wait(&sh.s_full[st][cnt % SR], (uint32_t)(cnt / SR) & 1u);
@@ -1181,11 +1239,14 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
         const int grid = ctx->sm_count;
         rc = ragged_scratch(ctx, grid, &p.part_acc, &p.part_ml, &p.counters);
         if (rc != INF_OK) return rc;
-        CUtensorMap tq, tk, tv;
+        CUtensorMap tq, tq_light, tk, tv;
         {
             const uint64_t dims[3] = {D, (uint64_t)q_heads, (uint64_t)tokens}, strides[2] = {D * 2, (uint64_t)q_heads * D * 2};
             const uint32_t box[3] = {64, (uint32_t)group, (uint32_t)p.stream_tokens};
             rc = inf_make_tmap(ctx, q_f16, 3, dims, strides, box, &tq);
+            if (rc != INF_OK) return rc;
+            const uint32_t light_box[3] = {64, (uint32_t)group, (uint32_t)(p.light_tokens > 0 ? p.light_tokens : 1)};
+            rc = inf_make_tmap(ctx, q_f16, 3, dims, strides, light_box, &tq_light);
             if (rc != INF_OK) return rc;
         }
         {
@@ -1202,7 +1263,7 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
         }
         {
             inf_prof_scope prof(ctx, "ragged_attention_kernel");
-            INF_CUDA(ctx, inf_launch_pdl(ragged_attention_kernel, dim3((unsigned)grid), dim3(THREADS), (size_t)SMEM_BYTES, ctx->stream, tq, tk, tv, p));
+            INF_CUDA(ctx, inf_launch_pdl(ragged_attention_kernel, dim3((unsigned)grid), dim3(THREADS), (size_t)SMEM_BYTES, ctx->stream, tq, tq_light, tk, tv, p));
         }
         return INF_OK;
     });
