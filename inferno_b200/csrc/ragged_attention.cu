@@ -76,7 +76,7 @@ struct Found {
 struct Shared {
     uint64_t q_full[2], q_free[2], k_full[KS], v_full[VS];
     uint64_t s_full[2][SR];   // S of a stream's tile is in TMEM, PV of its tile before has retired
-    uint64_t p_full[2][2];    // keys 0-63 / 64-127 of a stream's P are in TMEM
+    uint64_t p_full[2][2];    // keys 64-127 / 0-63 of a stream's P are in TMEM
     uint64_t o_ready[2][SR];  // PV of a stream's tile has retired
     uint64_t item_full[RING], item_free[RING];
     uint64_t v_patched[VS];   // dead slots of the V tile in this ring slot have been cleared
@@ -427,9 +427,9 @@ __device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, 
     const int lane = threadIdx.x & 31;
     if (masked) mask_scores(col_s, k0, qpos, first_key);
     float top = -INFINITY;
+    uint32_t x[64];
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {
-        uint32_t x[64];
         tmem_ld32(col_s + h * 64, x);
         tmem_ld32(col_s + h * 64 + 32, x + 32);
         tc_wait_ld64(x);
@@ -456,17 +456,20 @@ __device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, 
     }
     uint64_t sums[2] = {0, 0};
 #pragma unroll 1
-    for (int h = 0; h < 2; ++h) {
-        uint32_t x[64], packed[32];
-        tmem_ld32(col_s + h * 64, x);
-        tmem_ld32(col_s + h * 64 + 32, x + 32);
-        tc_wait_ld64(x);
+    for (int h = 0;; ++h) {  // keys 64-127, which are there, then keys 0-63
+        uint32_t packed[32];
         exponentials(x, p.scale_log2, m_used, packed, sums);
-        tmem_st32(col_s + h * 32, packed);  // over columns of S that have been read
+        tmem_st32(col_s + (h == 0 ? 64 : 0), packed);  // over columns of S that have been read
+        if (h == 0) {
+            tmem_ld32(col_s, x);
+            tmem_ld32(col_s + 32, x + 32);
+        }
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_full[st][h]);  // 64 keys of P are there: their PV may start
+        if (h == 1) break;
+        tc_wait_ld64(x);
     }
     float a, b;
     unpack_f32x2(add_f32x2(sums[0], sums[1]), a, b);
@@ -518,17 +521,17 @@ __device__ __forceinline__ void softmax_tile_few(Shared& sh, const RaggedParams&
     }
     float sum = 0.f;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < 2; ++half) {  // keys 64-127 first
         uint32_t y[16];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float a = ex2_approx(fmaf(__uint_as_float(x[4 * (half * 8 + k)]), p.scale_log2, -m_used));
-            const float b = ex2_approx(fmaf(__uint_as_float(x[4 * (half * 8 + k) + 1]), p.scale_log2, -m_used));
+            const float a = ex2_approx(fmaf(__uint_as_float(x[4 * (8 - half * 8 + k)]), p.scale_log2, -m_used));
+            const float b = ex2_approx(fmaf(__uint_as_float(x[4 * (8 - half * 8 + k) + 1]), p.scale_log2, -m_used));
             sum += a + b;
             y[2 * k] = pack_half2(a, b);
             y[2 * k + 1] = 0u;  // lanes 8-15 hold no row
         }
-        tmem_st_16x128_x8(col_s + half * 32, y);
+        tmem_st_16x128_x8(col_s + 64 - half * 64, y);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -913,11 +916,22 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     q_parity ^= 2u;
                 }
                 // step w: PV of tile w - 2 of the steps, then S of tile w
+                auto scores = [&](int st, uint32_t col_s, bool last) {
+                    const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) {
+                        const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
+                        umma_ss(col_s, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
+                    }
+                    tc_commit(&sh.s_full[st][st ? s_at[1].slot : s_at[0].slot]);
+                    if (last) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
+                };
 #pragma unroll 1
                 for (int w = 0; w < steps + 2; ++w) {
                     const int st = w & 1;
                     const uint32_t col_s = tb + COL_S + st * BN, col_o = tb + COL_O + st * D;
-                    const bool new_tile = shared_rows || st == 0;
+                    const bool new_tile = shared_rows || st == 0, more = w < steps;
+                    const bool last = w + 1 == steps || (!shared_rows && w + 2 == steps);
                     if (w >= 2) {
                         if (new_tile) {
                             uniform_wait(&sh.v_full[v_at.slot], v_at.parity, tries);
@@ -928,43 +942,42 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                             v_lo = v_lo0 + v_at.slot * (TILE_BYTES >> 4);
                             v_at.step();
                         }
-#pragma unroll 1
-                        for (int half = 0; half < 2; ++half) {  // the halves of P arrive separately
-                            uniform_wait(&sh.p_full[st][half], (p_parity >> st) & 1u, tries);
-                            tc_fence_after();
-                            if (elect_one()) {
+                        // the halves of P arrive separately
+                        uniform_wait(&sh.p_full[st][0], (p_parity >> st) & 1u, tries);
+                        tc_fence_after();
+                        if (elect_one()) {
 #pragma unroll
-                                for (int kk = 0; kk < 4; ++kk)
-                                    umma_ts(col_o, col_s + half * 32 + kk * 8, umma_desc_pack(v_lo + (half * 4 + kk) * (2048 >> 4), hi), idesc_o,
-                                            kk > 0 || half > 0 || w >= 4);
-                            }
-                            __syncwarp();
+                            for (int kk = 0; kk < 4; ++kk)
+                                umma_ts(col_o, col_s + 64 + kk * 8, umma_desc_pack(v_lo + (4 + kk) * (2048 >> 4), hi), idesc_o, kk > 0 || w >= 4);
                         }
+                        __syncwarp();
+                    }
+                    if (more && new_tile) {
+                        uniform_wait(&sh.k_full[k_at.slot], k_at.parity, tries);
+                        k_lo = k_lo0 + k_at.slot * (TILE_BYTES >> 4);
+                        k_at.step();
+                    }
+                    if (w >= 2) {
+                        uniform_wait(&sh.p_full[st][1], (p_parity >> st) & 1u, tries);
+                        tc_fence_after();
                         p_parity ^= 1u << st;
-                        if (elect_one()) tc_commit(&sh.o_ready[st][st ? o_at[1].slot : o_at[0].slot]);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk)
+                                umma_ts(col_o, col_s + kk * 8, umma_desc_pack(v_lo + kk * (2048 >> 4), hi), idesc_o, 1u);
+                            tc_commit(&sh.o_ready[st][st ? o_at[1].slot : o_at[0].slot]);
+                            if (more) scores(st, col_s, last);
+                        }
                         __syncwarp();
                         if (st)
                             o_at[1].step();
                         else
                             o_at[0].step();
-                    }
-                    if (w < steps) {
-                        if (new_tile) {
-                            uniform_wait(&sh.k_full[k_at.slot], k_at.parity, tries);
-                            k_lo = k_lo0 + k_at.slot * (TILE_BYTES >> 4);
-                            k_at.step();
-                        }
-                        const uint32_t q_lo = q_lo0 + (shared_rows ? 0u : (uint32_t)st * (TILE_BYTES >> 4));
-                        if (elect_one()) {
-#pragma unroll
-                            for (int kk = 0; kk < 8; ++kk) {
-                                const uint32_t off = (uint32_t)((kk >> 2) * BLK_BYTES + (kk & 3) * 32) >> 4;
-                                umma_ss(col_s, umma_desc_pack(q_lo + off, hi), umma_desc_pack(k_lo + off, hi), idesc_s, kk > 0);
-                            }
-                            tc_commit(&sh.s_full[st][st ? s_at[1].slot : s_at[0].slot]);
-                            if (w + 1 == steps || (!shared_rows && w + 2 == steps)) tc_commit(&sh.q_free[shared_rows ? 0 : st]);  // the last S that reads this Q
-                        }
+                    } else if (more) {
+                        if (elect_one()) scores(st, col_s, last);
                         __syncwarp();
+                    }
+                    if (more) {
                         if (st)
                             s_at[1].step();
                         else
