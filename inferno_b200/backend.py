@@ -261,14 +261,14 @@ class CudaBackend:
 
     def _mine(self, what: str, dtype, *tensors, contiguous: bool = True):
         """The arguments of one call: on this context's GPU, of one dtype, contiguous unless the call takes strides."""
+        device = self.device
         for t in tensors:
-            if t is None:
+            if t is None or (t.device == device and t.dtype is dtype and (not contiguous or t.is_contiguous())):
                 continue
             self._here(what, t)
-            if t.dtype != dtype:
+            if t.dtype is not dtype:
                 raise InfernoError(L.INF_E_DTYPE, f"{what}: expected {dtype}, got {t.dtype}")
-            if contiguous and not t.is_contiguous():
-                raise InfernoError(L.INF_E_ARG, f"{what}: tensor must be contiguous")
+            raise InfernoError(L.INF_E_ARG, f"{what}: tensor must be contiguous")
 
     def _new(self, shape, dtype) -> torch.Tensor:
         """Memory for an output that the library's stream writes: from that stream's pool, so that no other stream's

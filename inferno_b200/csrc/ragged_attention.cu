@@ -22,10 +22,10 @@
 //   warp 9           issues every MMA, in the order  S(0) S(1) | PV(0) S(2) | PV(1) S(3) | ...  over the streams' tiles in turn
 //   warp 10          loads the V ring (TMA)
 //   warp 11          loads Q
-// S = Q K^T is an SS MMA (M128 N128 K16), O += P V a TS MMA: P, packed fp16, lies over the first half of its own S in TMEM,
-// V is read MN-major straight from its [key][dim] tile.  One thread's MMAs run in order, so S of a stream's next tile, issued
-// behind PV, may overwrite that P, and its barrier also says that PV has retired: a softmax warp waits for one barrier per
-// tile, and while it works on one stream the tensor cores have PV and S of the other.
+// S = Q K^T is an SS MMA (M128 N128 K16), O += P V a TS MMA: P, packed fp16, lies over its own S in TMEM, 64 keys of it over
+// the columns 0-31 and 64 over 64-95, V is read MN-major straight from its [key][dim] tile.  One thread's MMAs run in order,
+// so S of a stream's next tile, issued behind PV, may overwrite that P, and its barrier also says that PV has retired: a
+// softmax warp waits for one barrier per tile, and while it works on one stream the tensor cores have PV and S of the other.
 // TMEM: S 128 columns and O 128 columns per stream.  Shared memory: Q 2 x 32 KB, K 3 x 32 KB, V 2 x 32 KB.
 //
 // Rows of few items fill few of the 128 lanes, and a warp's exponentials go through one of the four special-function
@@ -33,6 +33,16 @@
 // threads (16x256 TMEM shape): 32 exponentials a thread and tile instead of 128 on one warp.  Their MMAs are of M64, whose
 // rows are lanes 0-15 of each quarter: a batch of decodes holds the GPU at its power limit, and half the multiplications
 // leave the clock 8 % higher (139 -> 133 us).
+//
+// What bounds it, and what it takes on a B200 (a floor is the keys' bytes at the measured copy bandwidth or the products at the
+// measured cuBLAS rate; the first figure from a cool GPU, the second held at its power limit):
+//   32 decodes of 1 024-16 384 keys, 48 / 8 heads   125, 130 us   floor 114: memory
+//   24 sequences of 6 drafts, 64 / 8 heads           80, 82        60: memory, then the CTAs' start (5 us), unequal SMs, the join
+//   46 decodes and two chunks of 1 024, 48 / 8      148, 170       84: the chunks' tiles (softmax and MMAs in turn), joins
+//   40 decodes and a chunk of 777, window 512        50, 50        10: five tiles an item, so its start and end; no two parts alike
+//   a chunk of 4 096 on 8 192 keys, 48 / 8          935, 1 030    626: a stream's tile takes softmax 2 100 + MMAs 1 300 cycles,
+//                                                                  and the other stream covers half of that
+//   one decode of 100 keys                            11 in a graph: launch, cold code, a chain of five waits
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -47,10 +57,7 @@ namespace {
 constexpr int D = 128;
 constexpr int BM = 128, BN = RAGGED_TILE;
 constexpr int THREADS = 384;
-#ifndef RKS
-#define RKS 3
-#endif
-constexpr int KS = RKS, VS = 5 - RKS;  // tiles in the K and V rings
+constexpr int KS = 3, VS = 2;          // tiles in the K and V rings
 constexpr int SR = 4;                  // rotation of the barriers that free their slots: one is looked at up to three tiles late
 constexpr int TILE_BYTES = BN * D * 2;  // also the bytes of a stream's Q
 constexpr int BLK_BYTES = BN * 128;    // [128 rows][64 columns] with the 128-byte swizzle
@@ -81,6 +88,7 @@ struct Shared {
     uint64_t item_full[RING], item_free[RING];
     uint64_t v_patched[VS];   // dead slots of the V tile in this ring slot have been cleared
     uint64_t join[2];         // shared rows: stream 1's maxima and sums are in ml / its O has been read
+    uint64_t drained;         // every MMA has retired
     uint64_t part_bar, flag_bar;  // the CTA's pieces are in scratch / whether they were their items' last
     uint32_t tmem;
     int last_piece[2];
@@ -420,8 +428,9 @@ __device__ __forceinline__ float max_of(const uint32_t* x) {
                 fmaxf(__uint_as_float(x[62]), __uint_as_float(x[63])));
 }
 
-// thread = row.  Loops over the halves of the row, read from TMEM twice, keep the code short: three warps with different
-// code share a scheduler's instruction cache, and the thread that issues the MMAs must not wait for its instructions.
+// thread = row.  Loops over the halves of the row keep the code short: three warps with different code share a scheduler's
+// instruction cache, and the warp that issues the MMAs must not wait for its instructions.  The maximum leaves keys 64-127 in
+// registers; their weights come first, and the scores of keys 0-63 are read again behind them.
 __device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, uint32_t col_s, uint32_t col_o, int st, int k0,
                                              int qpos, int first_key, bool masked, bool valid, bool first, float& m_used, float& l) {
     const int lane = threadIdx.x & 31;
@@ -659,6 +668,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             mbar_init(&sh.item_full[i], 1);
             mbar_init(&sh.item_free[i], 11);  // every warp but the one that writes
         }
+        mbar_init(&sh.drained, 1);
         mbar_init(&sh.part_bar, 8);
         mbar_init(&sh.flag_bar, 1);
         mbar_fence_init();
@@ -987,6 +997,9 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 alive = __all_sync(0xffffffffu, tries != 0);
                 if (!alive) break;
             }
+            if (elect_one()) tc_commit(&sh.drained);  // also after a wait that gave up: TMEM is freed behind the last MMA
+            __syncwarp();
+            alive = warp_wait(&sh.drained, 0) && alive;
         }
         if (!alive && lane == 0) atomicOr(p.status, INF_STATUS_WAIT_TIMEOUT);
     } else {
