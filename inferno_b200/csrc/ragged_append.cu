@@ -10,7 +10,6 @@
 
 #include "common.cuh"
 #include "ptx.cuh"
-#include "rows.cuh"
 
 using namespace inf;
 

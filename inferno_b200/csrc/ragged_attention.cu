@@ -1230,7 +1230,7 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
         if (!(scale <= 1e15f)) return inf_fail(ctx, INF_E_CONFIG, "%s: scale must be finite and at most 1e15", what);
         if (out_dtype != INF_DTYPE_F32 && out_dtype != INF_DTYPE_F16)
             return inf_fail(ctx, INF_E_DTYPE, "%s: output dtype must be f32 or f16", what);
-        int rc = inf_validate_table(ctx, table, pool->num_pages, pool->page_size, 0, what, sliding_window, 1);
+        int rc = inf_validate_table(ctx, table, pool->num_pages, pool->page_size, 0, what, sliding_window, 0);
         if (rc != INF_OK) return rc;
         if (tokens == 0) return INF_OK;
         if (!q_f16 || !q_starts || !out) return inf_fail(ctx, INF_E_ARG, "%s: null pointer", what);

@@ -9,7 +9,6 @@
 
 #include "common.cuh"
 #include "fp8.cuh"
-#include "rows.cuh"
 
 namespace {
 
@@ -86,6 +85,41 @@ __global__ void qk_norm_rope_pair_kernel(const float* __restrict__ q, const floa
 // row of 128 values is held by 16 threads, eight consecutive values each, so that every load and store is 16 bytes
 // per thread and 256 contiguous bytes per row.  The half-split rotation partner (d +- rotary/2) sits rotary/16 lanes
 // away in the same 16-lane group.
+// eight consecutive input values as they lie in memory (one 16-byte piece for fp16, two for f32) ...
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = reinterpret_cast<const float4*>(p)[0];
+        b = reinterpret_cast<const float4*>(p)[1];
+    }
+    __device__ __forceinline__ void to_f32(float (&x)[8]) const {
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    }
+};
+template <>
+struct Raw8<__half> {
+    uint4 raw;
+    __device__ __forceinline__ void load(const __half* p) { raw = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void to_f32(float (&x)[8]) const {
+        const __half2* h = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = __half22float2(h[j]);
+            x[2 * j] = f.x, x[2 * j + 1] = f.y;
+        }
+    }
+};
+__device__ __forceinline__ void st8_as_f16(__half* p, const float (&x)[8]) {
+    uint4 raw;
+    __half2* h = reinterpret_cast<__half2*>(&raw);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+    *reinterpret_cast<uint4*>(p) = raw;
+}
+
 // FP8: the pools hold E4M3FN bytes, stored byte = encode(x / scale) with one scale per tensor
 // (fp8_attention_kernels.metal:227-263); the roped keys and the values of the call's tokens are also written out as
 // fp16 (cur_k_out / cur_v_out), because attention reads the current tokens at full precision, not through the cache.

@@ -284,6 +284,22 @@ def test_attention_ragged_keeps_nothing_of_the_call_before(be, past, new, Hq, Hk
     be.device_flush()
 
 
+def test_attention_ragged_pages_below_the_window_given_back(be):
+    """Host mirrors check the pages that a row can see and no others: the first row sees keys from past + 1 - window on."""
+    from inferno_b200 import InfernoError
+    b = Batch(be.device, [95, 200], [1, 3], 12, 2, 16, seed=22, window=64)  # lowest visible keys 32 and 137
+    want = b.check(be)
+    b.pages[0, :2] = -1
+    b.pages[1, :8] = -1
+    pool = be.kv_pool(b.k, b.v)
+    got = be.gqa_attention_ragged(b.q, pool, be.page_table(b.pages, b.past_lens), b.q_starts, sliding_window=64)
+    be.device_flush()
+    assert torch.equal(got, want)
+    b.pages[0, 2] = -1
+    with pytest.raises(InfernoError, match="page"):
+        be.gqa_attention_ragged(b.q, pool, be.page_table(b.pages, b.past_lens), b.q_starts, sliding_window=64)
+
+
 @pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
 def test_attention_ragged_rows_at_odd_sixteen_bytes(be, out_dtype):
     """Queries and output that begin 16 bytes into a 32-byte sector."""
