@@ -256,27 +256,29 @@ class CudaBackend:
     def _here(self, what: str, *tensors):
         """The tensors behind a descriptor: on this context's GPU."""
         for t in tensors:
-            if t.device != self.device:
+            if t.get_device() != self.device.index:
                 raise InfernoError(L.INF_E_ARG, f"{what}: tensor on {t.device}, the context is on {self.device}")
 
     def _mine(self, what: str, dtype, *tensors, contiguous: bool = True):
         """The arguments of one call: on this context's GPU, of one dtype, contiguous unless the call takes strides."""
-        device = self.device
+        gpu = self.device.index
         for t in tensors:
-            if t is None or (t.device == device and t.dtype is dtype and (not contiguous or t.is_contiguous())):
+            if t is None or (t.dtype is dtype and t.get_device() == gpu and (not contiguous or t.is_contiguous())):
                 continue
             self._here(what, t)
             if t.dtype is not dtype:
                 raise InfernoError(L.INF_E_DTYPE, f"{what}: expected {dtype}, got {t.dtype}")
             raise InfernoError(L.INF_E_ARG, f"{what}: tensor must be contiguous")
 
-    def _new(self, shape, dtype) -> torch.Tensor:
+    def _new(self, shape, dtype, like: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Memory for an output that the library's stream writes: from that stream's pool, so that no other stream's
-        pending work still uses it."""
-        if self.stream.cuda_stream == torch.cuda.current_stream(self.device.index).cuda_stream:
-            return torch.empty(shape, dtype=dtype, device=self.device)
-        with torch.cuda.stream(self.stream):
-            return torch.empty(shape, dtype=dtype, device=self.device)
+        pending work still uses it.  `like`: a tensor of that shape on this GPU, which torch copies in less time."""
+        if self.stream.cuda_stream != torch._C._cuda_getCurrentRawStream(self.device.index):
+            with torch.cuda.stream(self.stream):
+                return torch.empty(shape, dtype=dtype, device=self.device)
+        if like is not None:
+            return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+        return torch.empty(shape, dtype=dtype, device=self.device)
 
     # ------------------------------------------------------------------ descriptors
     def prepare_rope_table(self, inv_freq, rotary_dim: int, attention_factor: float) -> L.RopeTable:  # backend.rs:1227
@@ -376,11 +378,11 @@ class CudaBackend:
         self._here("device_index_append", index.pages)
         self._mine("device_index_append", torch.int32, new_tokens, batch.past_lens, batch.q_starts, batch.positions, batch.slots)
         seqs = index.desc.max_seqs
-        if new_tokens.shape != (seqs,) or batch.past_lens.shape != (seqs,) or batch.q_starts.shape != (seqs + 1,) \
-                or batch.positions.shape != batch.slots.shape:
+        tokens = batch.positions.numel()
+        if new_tokens.shape != (seqs,) or batch.past_lens.numel() != seqs or batch.q_starts.numel() != seqs + 1 or batch.slots.numel() != tokens:
             raise InfernoError(L.INF_E_SHAPE, f"device_index_append: the index has {seqs} sequences, got {tuple(new_tokens.shape)} lengths")
         self._check(self._lib.inf_device_index_append(
-            self._ctx, C.byref(index.desc), new_tokens.data_ptr(), batch.positions.numel(), batch.past_lens.data_ptr(),
+            self._ctx, C.byref(index.desc), new_tokens.data_ptr(), tokens, batch.past_lens.data_ptr(),
             batch.q_starts.data_ptr(), batch.positions.data_ptr(), batch.slots.data_ptr()))
         return batch
 
@@ -410,19 +412,25 @@ class CudaBackend:
                                               f"{tuple(positions.shape)}, slots {tuple(slots.shape)} do not fit {hkv} KV heads of {d}")
         if any(w is not None and w.shape != (d,) for w in (q_norm, k_norm)):
             raise InfernoError(L.INF_E_SHAPE, f"{what}: norm weights must have {d} values")
-        for t in (q, k, v):
-            if T and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != d)):
+        strides = []  # a single token's is never used: any tensor may stand there
+        for t, heads in ((q, Hq), (k, hkv), (v, hkv)):
+            if T > 1 and not t.is_contiguous():
+                token, head, value = t.stride()
+                if value != 1 or (heads > 1 and head != d):
+                    raise InfernoError(L.INF_E_ARG, f"{what}: the heads of a token must be contiguous")
+                strides.append(token)
+            elif T == 1 and not t.is_contiguous() and not t[0].is_contiguous():
                 raise InfernoError(L.INF_E_ARG, f"{what}: the heads of a token must be contiguous")
+            else:
+                strides.append(heads * d)
         if out is None:
-            out = self._new((T, Hq, d), torch.float16)
+            out = self._new((T, Hq, d), torch.float16, q)
         else:
             self._mine(what, torch.float16, out)
             if out.shape != (T, Hq, d):
                 raise InfernoError(L.INF_E_SHAPE, f"{what}: out must be {(T, Hq, d)}, got {tuple(out.shape)}")
-        # a single token's stride is never used: any tensor may stand there
-        qs, ks, vs = ((t.stride(0) if T > 1 else t.shape[1] * d) for t in (q, k, v))
         self._check(self._lib.inf_rope_append_gqa_ragged(
-            self._ctx, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs,
+            self._ctx, q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides,
             L.DTYPE_F32 if q.dtype == torch.float32 else L.DTYPE_F16, q_norm.data_ptr() if q_norm is not None else None,
             k_norm.data_ptr() if k_norm is not None else None, eps, C.byref(rope) if rope is not None else None,
             C.byref(pool.desc), positions.data_ptr(), slots.data_ptr(), T, Hq, out.data_ptr()))
@@ -445,7 +453,7 @@ class CudaBackend:
         if gate is not None and gate.shape != (T, Hq):
             raise InfernoError(L.INF_E_SHAPE, f"{what}: gate must be {(T, Hq)}, got {tuple(gate.shape)}")
         if out is None:
-            out = self._new((T, Hq, D), out_dtype)
+            out = self._new((T, Hq, D), out_dtype, q_f16)
         if out.shape != q_f16.shape:
             raise InfernoError(L.INF_E_SHAPE, f"{what}: out must be {(T, Hq, D)}, got {tuple(out.shape)}")
         if out.dtype not in (torch.float32, torch.float16):
