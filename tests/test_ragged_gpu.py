@@ -300,6 +300,45 @@ def test_attention_ragged_pages_below_the_window_given_back(be):
         be.gqa_attention_ragged(b.q, pool, be.page_table(b.pages, b.past_lens), b.q_starts, sliding_window=64)
 
 
+def test_a_pool_beyond_32_bits(be):
+    """Pages whose rows lie more than 2^32 values into the pools: the same bits as in a pool of a few pages."""
+    Hq, Hkv, P, past, new = 48, 8, 16, 70, 40
+    far = 2 ** 32 // (Hkv * P * 128)  # pages below the first one used
+    need = -(-(past + new) // P)
+    if torch.cuda.mem_get_info(be.device)[0] < 2 * (far + need) * Hkv * P * 256 + 2 ** 31:
+        pytest.skip("needs 18 GB of device memory")
+    g = torch.Generator(device=be.device).manual_seed(2)
+    cached = torch.randn((2, need, Hkv, P, 128), generator=g, device=be.device, dtype=torch.float16)
+    q, k, v = (torch.randn((new, h, 128), generator=g, device=be.device) for h in (Hq, Hkv, Hkv))
+    rope = be.prepare_rope_table(torch.ones(64) / (1 + torch.arange(64)), 128, 1.0)
+    outs = []
+    for first in (0, far):
+        pools = [torch.empty((first + need, Hkv, P, 128), dtype=torch.float16, device=be.device) for _ in range(2)]
+        for pool, rows in zip(pools, cached):
+            pool[first:] = rows
+        pool = be.kv_pool(*pools)
+        positions = past + torch.arange(new, dtype=torch.int32, device=be.device)
+        q16 = be.rope_append_gqa_ragged(q, k, v, rope, pool, positions, positions + first * P)
+        table = be.page_table(first + torch.arange(need, dtype=torch.int32, device=be.device)[None], ints(be, [past]), validate_on_host=False)
+        outs.append((be.gqa_attention_ragged(q16, pool, table, ints(be, [0, new])), pools[0][first:].clone(), pools[1][first:].clone()))
+        be.device_flush()
+        del pool, pools
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_attention_ragged_without_new_tokens(be):
+    """A step in which no sequence has a token writes nothing, before and after one that cuts items over many CTAs."""
+    b = Batch(be.device, [30000, 500], [1, 30], 12, 2, 16, seed=23)
+    pool, table = be.kv_pool(b.k, b.v), be.page_table(b.pages, b.past_lens, validate_on_host=False)
+    out = torch.full(b.q.shape, 7.0, dtype=torch.float16, device=be.device)
+    for _ in range(2):
+        be.gqa_attention_ragged(b.q, pool, table, ints(be, [0, 0, 0]), out=out)
+        be.device_flush()
+        assert (out == 7).all()
+        b.check(be)
+
+
 @pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
 def test_attention_ragged_rows_at_odd_sixteen_bytes(be, out_dtype):
     """Queries and output that begin 16 bytes into a 32-byte sector."""
