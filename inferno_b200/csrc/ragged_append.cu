@@ -4,7 +4,7 @@
 //     x' = x w / sqrt(mean x^2 + eps);  (a, b) -> (a cos - b sin, b cos + a sin) for the pairs (d, d + rotary / 2)
 //
 // HBM-bound: a token's q, k and v rows are read once and written once as fp16.  8192 tokens of 48 + 2 x 8 fp16 heads move
-// 268 MB in 51.5 us, 0.80 of the measured copy bandwidth; a single token takes 4.8 us of a graph.
+// 268 MB in 49.8 us, 0.82 of the measured copy bandwidth; a single token takes 4.1 us of a graph.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -22,7 +22,6 @@ struct AppendArgs {
     const void *q, *k, *v;
     long long q_stride, k_stride, v_stride;  // elements between tokens
     const float *qw, *kw, *inv_freq;
-    int rotary_dim;
     float factor, eps;
     __half *k_pool, *v_pool, *q_out;
     const int *positions, *slots;
@@ -47,9 +46,9 @@ struct Pieces;
 template <>
 struct Pieces<float> {
     float4 a, b;
-    __device__ __forceinline__ void load(const float* row, int ca, int cb) {
-        a = *reinterpret_cast<const float4*>(row + ca);
-        b = *reinterpret_cast<const float4*>(row + cb);
+    __device__ __forceinline__ void load(const float* at, int apart) {
+        a = *reinterpret_cast<const float4*>(at);
+        b = *reinterpret_cast<const float4*>(at + apart);
     }
     __device__ __forceinline__ void to_f32(uint64_t (&x)[2], uint64_t (&y)[2]) const {
         x[0] = pack_f32x2(a.x, a.y), x[1] = pack_f32x2(a.z, a.w), y[0] = pack_f32x2(b.x, b.y), y[1] = pack_f32x2(b.z, b.w);
@@ -58,9 +57,9 @@ struct Pieces<float> {
 template <>
 struct Pieces<__half> {
     uint2 a, b;
-    __device__ __forceinline__ void load(const __half* row, int ca, int cb) {
-        a = *reinterpret_cast<const uint2*>(row + ca);
-        b = *reinterpret_cast<const uint2*>(row + cb);
+    __device__ __forceinline__ void load(const __half* at, int apart) {
+        a = *reinterpret_cast<const uint2*>(at);
+        b = *reinterpret_cast<const uint2*>(at + apart);
     }
     static __device__ __forceinline__ uint64_t pair(uint32_t h) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
@@ -86,28 +85,30 @@ __device__ __forceinline__ uint64_t shfl_xor2(uint64_t v, int o) {
 // A warp works on one token, or with `parts` > 1 on every parts-th pair of its rows.  16 lanes hold a row, each four
 // values and their four rotation partners, so a rotation needs no other lane, its four cosines and sines stay in
 // registers for all rows, and a warp's 8-byte accesses still fill whole sectors.  Eight neighbouring values a lane need
-// eight shuffles a step for the partners and twice the cosines: 69 us instead of 51.5 for those 8192 tokens.  Rows are
+// eight shuffles a step for the partners and twice the cosines: 69 us instead of 49.8 for those 8192 tokens.  Rows are
 // requested AHEAD steps before they are worked on, the first ones before the position is known.  No barriers.
-template <typename T>
+template <typename T, int HALF>  // HALF: half the rotary dimension, what lies between partners
 __global__ void __launch_bounds__(THREADS, 8)
 rope_append_ragged_kernel(AppendArgs p) {
-    constexpr int AHEAD = sizeof(T) == 2 ? 3 : 2;  // what 64 registers hold
+    constexpr int AHEAD = sizeof(T) == 2 ? 4 : 2;  // what 64 registers hold
     inf_pdl_wait();
     inf_pdl_release();
     const int lane = threadIdx.x & 31, sub = lane & 15, upper = lane >> 4;
     const long long unit = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
     const int t = (int)(unit / p.parts), part = (int)(unit - (long long)t * p.parts);
     if (t >= p.tokens) return;
-    const int half = p.rotary_dim >> 1;
-    const bool turned = 4 * sub < half && p.inv_freq;
-    const int ca = 4 * sub < half ? 4 * sub : half + 4 * sub, cb = ca + (4 * sub < half ? half : 32);
+    // a row's rotated part is HALF / 4 lanes wide, what is left of it the others'
+    const bool turned = 4 * sub < HALF && p.inv_freq;
+    const int column = 4 * sub < HALF ? 4 * sub : HALF + 4 * sub;
     const int rows = p.q_heads + 2 * p.kv_heads, keys_from = p.q_heads, values_from = p.q_heads + p.kv_heads;
-    const T *q = (const T*)p.q + t * p.q_stride, *k = (const T*)p.k + t * p.k_stride, *v = (const T*)p.v + t * p.v_stride;
+    // rows are counted through queries, keys and values: each base stands where row 0 would
+    const T* q = (const T*)p.q + t * p.q_stride + column;
+    const T* k = (const T*)p.k + t * p.k_stride + column - (long long)keys_from * D;
+    const T* v = (const T*)p.v + t * p.v_stride + column - (long long)values_from * D;
     const int first = 2 * part + upper, stride = 2 * p.parts;  // this half-warp's rows
     auto request = [&](Pieces<T>& raw, int rr) {
         rr = min(rr, rows - 1);
-        raw.load(rr < keys_from ? q + (long long)rr * D
-                                : (rr < values_from ? k + (long long)(rr - keys_from) * D : v + (long long)(rr - values_from) * D), ca, cb);
+        raw.load((rr < keys_from ? q : (rr < values_from ? k : v)) + (long long)rr * D, HALF);
     };
     Pieces<T> raw[AHEAD];
 #pragma unroll
@@ -117,7 +118,11 @@ rope_append_ragged_kernel(AppendArgs p) {
     const bool stored = slot >= 0 && slot < p.slots_total;
     if (!stored && part == 0 && lane == 0) atomicOr(p.status, INF_STATUS_BAD_PAGE);
     const int page = stored ? slot / p.page_size : 0;
-    const long long pool_row = ((long long)page * p.kv_heads * p.page_size + (slot - page * p.page_size)) * D;
+    const long long pool_step = (long long)p.page_size * D;  // from a head to the next one of a page
+    const long long pool_row = ((long long)page * p.kv_heads * p.page_size + (slot - page * p.page_size)) * D + column;
+    __half* const q_to = p.q_out + (long long)t * p.q_heads * D + column;
+    __half* const k_to = p.k_pool + pool_row - keys_from * pool_step;
+    __half* const v_to = p.v_pool + pool_row - values_from * pool_step;
     uint64_t c[2] = {0, 0}, s[2] = {0, 0};
     if (p.inv_freq) {
         // the half-warps make two of the four each
@@ -148,7 +153,7 @@ rope_append_ragged_kernel(AppendArgs p) {
                     if (w && rr < values_from) {
                         const float scale = rsqrtf(sum * (1.0f / D) + p.eps);
                         const uint64_t scale2 = pack_f32x2(scale, scale);
-                        const float4 wa = *reinterpret_cast<const float4*>(w + ca), wb = *reinterpret_cast<const float4*>(w + cb);
+                        const float4 wa = *reinterpret_cast<const float4*>(w + column), wb = *reinterpret_cast<const float4*>(w + column + HALF);
                         x[0] = mul_f32x2(mul_f32x2(x[0], pack_f32x2(wa.x, wa.y)), scale2);
                         x[1] = mul_f32x2(mul_f32x2(x[1], pack_f32x2(wa.z, wa.w)), scale2);
                         y[0] = mul_f32x2(mul_f32x2(y[0], pack_f32x2(wb.x, wb.y)), scale2);
@@ -165,11 +170,9 @@ rope_append_ragged_kernel(AppendArgs p) {
                 }
             }
             if (rr < rows && (rr < keys_from || stored)) {
-                __half* to = rr < keys_from ? p.q_out + ((long long)t * p.q_heads + rr) * D
-                             : rr < values_from ? p.k_pool + pool_row + (long long)(rr - keys_from) * p.page_size * D
-                                                : p.v_pool + pool_row + (long long)(rr - values_from) * p.page_size * D;
-                st4_as_f16(to + ca, x);
-                st4_as_f16(to + cb, y);
+                __half* to = (rr < keys_from ? q_to : (rr < values_from ? k_to : v_to)) + rr * (rr < keys_from ? (long long)D : pool_step);
+                st4_as_f16(to, x);
+                st4_as_f16(to + HALF, y);
             }
         }
     }
@@ -220,9 +223,11 @@ extern "C" int32_t inf_rope_append_gqa_ragged(inf_ctx* ctx, const void* q, const
         int parts = 1;
         while (parts < 8 && (long long)tokens * parts < 8LL * ctx->sm_count) parts *= 2;
         AppendArgs p{q, k, v, q_stride, k_stride, v_stride, q_norm_weight, k_norm_weight, rope ? rope->inv_freq : nullptr,
-                     rope ? rope->rotary_dim : 64, rope ? rope->attention_factor : 1.0f, eps, (__half*)pool->k, (__half*)pool->v,
+                     rope ? rope->attention_factor : 1.0f, eps, (__half*)pool->k, (__half*)pool->v,
                      (__half*)q_out_f16, positions, slots, tokens, parts, q_heads, pool->kv_heads, pool->page_size, pool->num_pages * pool->page_size, ctx->status};
-        auto kernel = in_dtype == INF_DTYPE_F16 ? rope_append_ragged_kernel<__half> : rope_append_ragged_kernel<float>;
+        const bool wide = rope && rope->rotary_dim == 128, f16 = in_dtype == INF_DTYPE_F16;
+        auto kernel = f16 ? (wide ? rope_append_ragged_kernel<__half, 64> : rope_append_ragged_kernel<__half, 32>)
+                          : (wide ? rope_append_ragged_kernel<float, 64> : rope_append_ragged_kernel<float, 32>);
         const long long blocks = ((long long)tokens * parts + THREADS / 32 - 1) / (THREADS / 32);
         INF_CUDA(ctx, inf_launch_pdl(kernel, dim3((unsigned)blocks), dim3(THREADS), 0, ctx->stream, p));
         return INF_OK;
