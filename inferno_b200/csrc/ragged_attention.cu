@@ -214,12 +214,12 @@ __device__ __forceinline__ bool find_part(const RaggedParams& p, Shared& sh) {
             kvh = place.kvh;
             item = place.i;
             const int first_tile = h.first_tile(item), end_tile = h.end_tile(item);
+            tile = place.tile_of(h, line, c + e);
             for (int k0 = place.first_cut(line);; k0 += 32) {
                 const int t = place.tile_of(h, line, k0 + lane);
                 const uint32_t in = __ballot_sync(0xffffffffu, t > first_tile && t < end_tile);
                 if (in && inside == 0) first = k0 + __ffs(in) - 1;
                 inside += __popc(in);
-                if (c + e >= k0 && c + e < k0 + 32) tile = __shfl_sync(0xffffffffu, t, c + e - k0);
                 if (__any_sync(0xffffffffu, t == end_tile)) break;  // these cuts reach the item's end
             }
         }
@@ -314,7 +314,8 @@ __device__ __forceinline__ int dead_slots(const RaggedParams& p, const Item& it,
 
 // Slots of key tile t below the lowest key any row sees, in the box that brings that key.
 __device__ __forceinline__ int dead_below(const RaggedParams& p, const Item& it, int t) {
-    return it.lowest > t * BN ? (it.lowest - t * BN) % p.box_rows : 0;
+    const int under = it.lowest - t * BN;
+    return under > 0 && under < BN ? under % p.box_rows : 0;
 }
 
 // Who reads a tile last: (stream, that stream's count of tiles) of the last three tiles, so that a producer knows which

@@ -300,6 +300,22 @@ def test_attention_ragged_pages_below_the_window_given_back(be):
         be.gqa_attention_ragged(b.q, pool, be.page_table(b.pages, b.past_lens), b.q_starts, sliding_window=64)
 
 
+@pytest.mark.parametrize("past,new,Hq,Hkv,window", [
+    ([4150], [42], 6, 1, 0),       # 33 parts: the last two cuts move to the item's end, one in each 32 of them
+    ([9000], [42], 6, 1, 4150),    # the same in a window
+    ([8310], [42], 6, 1, 0),       # 65 parts
+    ([12440, 3], [42, 1], 6, 1, 0),
+])
+def test_attention_ragged_items_of_many_pieces(be, past, new, Hq, Hkv, window):
+    b = Batch(be.device, past, new, Hq, Hkv, 16, seed=24, window=window)
+    assert torch.equal(b.check(be), b.check(be))
+
+
+@pytest.mark.parametrize("past", list(range(4090, 4230, 10)) + list(range(8200, 8400, 20)))
+def test_attention_ragged_around_whole_warps_of_cuts(be, past):
+    Batch(be.device, [past, 20], [42, 2], 6, 1, 16, seed=past).check(be)
+
+
 def test_a_pool_beyond_32_bits(be):
     """Pages whose rows lie more than 2^32 values into the pools: the same bits as in a pool of a few pages."""
     Hq, Hkv, P, past, new = 48, 8, 16, 70, 40
