@@ -12,11 +12,13 @@ constexpr int RAGGED_TILE = 128;  // keys of a tile
 // Costs, in halves of a key of a light item.  A key of an item of two streams costs two and a half times as much (with twice:
 // two chunks of 1 024 among 46 decodes 159 us instead of 148, a window of 512 49 instead of 51), of one stream of many rows one
 // and a half times (items of 33 to 64 rows count as light: 24 sequences' drafts 95 us as heavy ones, 82 as light); an item
-// costs some keys besides (256 light ones; with 192 or 384 the window takes 54 us); and a CTA's part is worth three tiles at
-// least, which also keeps two cuts of one item from falling on the same tile.  Cuts near an end of an item of two streams move
-// to it (RAGGED_SNAP; with one tile instead of two the window's items of five tiles fall apart: 68 us).
+// costs some keys besides (256 light ones; with 192 or 384 the window takes 54 us).  A CTA's part is worth a tile of two
+// streams at least, which keeps two cuts of one item from falling on the same tile, and no more, so that short decodes are
+// parts of their own (with three light tiles a decode of 100 keys and 8 heads was seven parts: 11.6 us instead of 9.3).  Cuts
+// near an end of an item of two streams move to it (RAGGED_SNAP; with one tile instead of two the window's items of five
+// tiles fall apart: 68 us).
 constexpr int RAGGED_ITEM_COST = 512;
-constexpr int RAGGED_MIN_PART = 2 * 3 * RAGGED_TILE;
+constexpr int RAGGED_MIN_PART = 5 * (RAGGED_TILE + 1);  // one key more: cuts are rounded
 constexpr int RAGGED_SNAP = 2;
 
 // The items of T tokens of one KV head of a sequence: n new tokens behind `past` cached ones, past + n at most 2^29.  An item
