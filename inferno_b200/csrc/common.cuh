@@ -48,6 +48,7 @@ struct inf_ctx {
     std::vector<void*> retired_workspaces;  // outgrown workspaces, kept until destroy: captured graphs may name them
     void* ragged_scratch = nullptr;  // pieces of cut items and their counters (ragged_attention.cu); fixed size
     int* ragged_counters = nullptr;   // its last sm_count words
+    int index_ctas = 0;               // most CTAs of a device index's cluster (device_index.cu); 0: not asked yet
     size_t dsa_scores_smem = 0;  // dynamic shared memory the tensor-core index-score kernel has been allowed so far
     int* status = nullptr;       // device int32[4]
     int* host_status = nullptr;  // pinned int32[4]

@@ -8,19 +8,19 @@
 // lengths restores the free list exactly.  Both are prefix sums over the batch; a few KB move, so what counts is the
 // length of the chain of dependent loads.
 //
-// A cluster of up to eight CTAs shares a call.  Each takes the prefix sums over the whole batch into its own shared
+// A cluster of up to sixteen CTAs shares a call.  Each takes the prefix sums over the whole batch into its own shared
 // memory, which is cheaper than waiting for another's, and then its share of the tokens and of the pages:
 // a search of the prefix sums gives the sequence, and a fresh page is read from the free list itself, not from the row
 // that another thread is writing.  The cluster's barrier stands between the last read of the lengths and their update.
-// An append and a truncate in a graph take 8.2 us for 32 decodes, 11.0 for 300 sequences of up to 9 new tokens, and 19.1
-// for 1000 of up to 127 (65 000 rows; one CTA alone: 94), of which the two launches are about 5.
+// An append and a truncate in a graph take 8.2 us for 32 decodes, 11.0 for 300 sequences of up to 9 new tokens, and 16.4
+// for 1000 of up to 127 (65 000 rows; eight CTAs 19.1, one alone 94), of which the two launches are about 5.
 #include "common.cuh"
 
 namespace {
 
 constexpr int THREADS = 1024;
 constexpr int WARPS = THREADS / 32;
-constexpr int MOST_CTAS = 8;
+constexpr int MOST_CTAS = 16;  // of a cluster; more than eight are not possible on every GPU
 constexpr int MOST_SEQS = 16384;  // three words of shared memory each
 
 struct IndexArgs {
@@ -233,21 +233,44 @@ device_index_truncate_kernel(IndexArgs a, const int* __restrict__ keep) {
     if (i0 == 0) *a.free_count = free_count + (int)gone.x;
 }
 
+// The CTAs that a cluster of these kernels may have on the context's GPU: sixteen where they fit, else the portable eight.
+int most_ctas(inf_ctx* ctx) {
+    if (ctx->index_ctas) return ctx->index_ctas;
+    const void* kernels[] = {(const void*)device_index_append_kernel<1>, (const void*)device_index_append_kernel<4>,
+                             (const void*)device_index_truncate_kernel};
+    int fits = MOST_CTAS;
+    for (const void* kernel : kernels) {
+        const int smem = (3 * MOST_SEQS + 2) * (int)sizeof(int);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(MOST_CTAS);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {MOST_CTAS, 1, 1};
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1)
+            fits = 8;
+    }
+    cudaGetLastError();  // what did not fit is no error
+    return ctx->index_ctas = fits;
+}
+
 // One cluster for `work` threads' work.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), long long work, int seqs, cudaStream_t stream, Args... args) {
+cudaError_t launch_cluster(inf_ctx* ctx, void (*kernel)(KArgs...), long long work, int seqs, Args... args) {
+    const int most = most_ctas(ctx);
     int ctas = 1;
-    while (ctas < MOST_CTAS && (long long)ctas * THREADS < work) ctas *= 2;
-    const size_t smem = (3 * (size_t)seqs + 2) * sizeof(int);
-    if (smem > 40 * 1024) {  // with the warps' sums more than a launch has without asking
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * MOST_SEQS + 2) * (int)sizeof(int));
-        if (e != cudaSuccess) return e;
-    }
+    while (ctas < most && (long long)ctas * THREADS < work) ctas *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
+    cfg.dynamicSmemBytes = (3 * (size_t)seqs + 2) * sizeof(int);
+    cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -307,8 +330,8 @@ extern "C" int32_t inf_device_index_append(inf_ctx* ctx, const inf_device_index*
         if (!new_tokens || !past_lens || !q_starts || !positions || !slots)
             return inf_fail(ctx, INF_E_ARG, "device_index_append: null pointer");
         if (max_tokens <= 0) return inf_fail(ctx, INF_E_SHAPE, "device_index_append: max_tokens must be positive, got %d", max_tokens);
-        const bool few = max_tokens <= MOST_CTAS * THREADS;
-        INF_CUDA(ctx, launch_cluster(few ? device_index_append_kernel<1> : device_index_append_kernel<4>, max_tokens, a.seqs, ctx->stream, a, new_tokens, max_tokens,
+        const bool few = max_tokens <= most_ctas(ctx) * THREADS;
+        INF_CUDA(ctx, launch_cluster(ctx, few ? device_index_append_kernel<1> : device_index_append_kernel<4>, max_tokens, a.seqs, a, new_tokens, max_tokens,
                                      past_lens, q_starts, positions, slots));
         return INF_OK;
     });
@@ -322,7 +345,7 @@ extern "C" int32_t inf_device_index_truncate(inf_ctx* ctx, const inf_device_inde
         if (rc != INF_OK) return rc;
         if (!keep_lens) return inf_fail(ctx, INF_E_ARG, "device_index_truncate: null pointer");
         // how many pages go is known on the GPU alone: four a sequence are expected
-        INF_CUDA(ctx, launch_cluster(device_index_truncate_kernel, 4LL * a.seqs, a.seqs, ctx->stream, a, keep_lens));
+        INF_CUDA(ctx, launch_cluster(ctx, device_index_truncate_kernel, 4LL * a.seqs, a.seqs, a, keep_lens));
         return INF_OK;
     });
 }

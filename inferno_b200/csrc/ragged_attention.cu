@@ -42,7 +42,7 @@
 //   40 decodes and a chunk of 777, window 512        50, 50        10: five tiles an item, so its start and end; no two parts alike
 //   a chunk of 4 096 on 8 192 keys, 48 / 8          935, 1 030    626: a stream's tile takes softmax 2 100 + MMAs 1 300 cycles,
 //                                                                  and the other stream covers half of that
-//   one decode of 100 keys                            11 in a graph: launch, cold code, a chain of five waits
+//   one decode of 100 keys                             9 in a graph: launch, cold code, a chain of five waits
 #include <cuda_fp16.h>
 #include <math.h>
 
