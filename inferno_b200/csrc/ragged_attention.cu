@@ -588,24 +588,14 @@ __device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& i
             sum = sum * ex2_approx(m - top) + sum2 * ex2_approx(m2 - top);
             m = top;
         };
-        float m = M_INIT, sum = 0.f;
-#pragma unroll 1
-        for (int q = lane % PIECES; q < it.pieces; q += PIECES) {
-            const float2 ml = max_and_sum(q);
-            merge(m, sum, ml.x, ml.y);
-        }
-#pragma unroll
-        for (int o = 1; o < PIECES; o <<= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
-            merge(m, sum, m2, sum2);
-        }
-        const float gain = (p.gate ? softplus(p.gate[out_mine]) : 1.0f) / sum;
+        const float gate = p.gate ? p.gate[out_mine] : 0.f;
+        float m = M_INIT, gain = 0.f;
         float4 acc[ROWS];
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
         for (int q = 0; q < it.pieces; q += PIECES) {
-            const float w = ex2_approx(max_and_sum(q + lane % PIECES).x - m) * gain;  // 0 behind the last piece
+            const float2 ml = max_and_sum(q + lane % PIECES);
             float4 v[PIECES][ROWS];
 #pragma unroll
             for (int e = 0; e < PIECES; ++e) {
@@ -615,6 +605,22 @@ __device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& i
                     for (int u = 0; u < ROWS; ++u) v[e][u] = __ldcg(base + row_in_piece(min(r0 + u * warps, all - 1)) * (D / 4));
                 }
             }
+            if (q == 0) {  // while the rows of the first pieces are on their way
+                m = ml.x;
+                float sum = ml.y;
+#pragma unroll 1
+                for (int r = PIECES + lane % PIECES; r < it.pieces; r += PIECES) {
+                    const float2 more = max_and_sum(r);
+                    merge(m, sum, more.x, more.y);
+                }
+#pragma unroll
+                for (int o = 1; o < PIECES; o <<= 1) {
+                    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
+                    merge(m, sum, m2, sum2);
+                }
+                gain = (p.gate ? softplus(gate) : 1.0f) / sum;
+            }
+            const float w = ex2_approx(ml.x - m) * gain;  // 0 behind the last piece
 #pragma unroll
             for (int e = 0; e < PIECES; ++e) {
                 if (q + e < it.pieces) {
