@@ -502,6 +502,30 @@ def test_captured_steps_replay_with_other_lengths(be):
     _run_steps(be, s, graph.replay, seed=2)
 
 
+def test_two_graphs_of_one_context_share_its_scratch(be):
+    """Two captured attentions, both with items cut over many CTAs, replayed in turn and twice in a row, with an eager call
+    between: each gives the bits of its own eager call."""
+    batches = [Batch(be.device, [30000, 7], [2, 90], 12, 2, 16, seed=30), Batch(be.device, [9000, 100, 5000], [130, 30, 1], 48, 8, 16, seed=31)]
+    want = [b.check(be) for b in batches]
+    outs = [torch.zeros_like(b.q) for b in batches]
+
+    def call(i):
+        b = batches[i]
+        be.gqa_attention_ragged(b.q, be.kv_pool(b.k, b.v), be.page_table(b.pages, b.past_lens, validate_on_host=False), b.q_starts, out=outs[i])
+
+    graphs = [be.capture_graph(lambda i=i: call(i)) for i in range(2)]
+    for order in ((0, 1), (1, 0), (0, 0), (1, 1)):
+        for o in outs:
+            o.zero_()
+        for i in order:
+            graphs[i].replay()
+        batches[0].check(be)
+        torch.cuda.synchronize()
+        for i in set(order):
+            assert torch.equal(outs[i][:batches[i].rows], want[i][:batches[i].rows])
+    be.device_flush()
+
+
 def test_two_contexts_on_two_streams(be):
     """Split attention of two contexts at the same time: neither sees the other's partial results."""
     from inferno_b200 import CudaBackend
