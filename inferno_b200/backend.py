@@ -8,7 +8,7 @@ memory and stream plumbing only: tensors are handed to the library as raw device
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Optional
 
 import torch
@@ -75,13 +75,31 @@ class DeviceIndex:
     desc: L.DeviceIndex
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class RaggedBatch:
-    """One step's layout, written by device_index_append; int32 tensors on the GPU."""
+    """One step's layout, written by device_index_append; contiguous int32 tensors on one GPU, checked here once."""
     past_lens: torch.Tensor  # [max_seqs] tokens cached before the step
     q_starts: torch.Tensor   # [max_seqs + 1] first row of each sequence
     positions: torch.Tensor  # [max_tokens], -1 behind the last token
     slots: torch.Tensor      # [max_tokens] page id * page_size + offset, -1 behind the last token
+    seqs: int = field(init=False)
+    gpu: int = field(init=False)
+    args: tuple = field(init=False, repr=False)  # max_tokens and the addresses, as the call takes them
+
+    def __post_init__(self):
+        tensors = (self.past_lens, self.q_starts, self.positions, self.slots)
+        for t in tensors:
+            if t.dtype != torch.int32:
+                raise InfernoError(L.INF_E_DTYPE, f"ragged batch: expected int32, got {t.dtype}")
+            if t.device.type != "cuda" or t.device != self.positions.device or not t.is_contiguous():
+                raise InfernoError(L.INF_E_ARG, "ragged batch: tensors must be contiguous and on one GPU")
+        seqs, tokens = self.past_lens.numel(), self.positions.numel()
+        if [t.shape for t in tensors] != [(seqs,), (seqs + 1,), (tokens,), (tokens,)]:
+            raise InfernoError(L.INF_E_SHAPE, "ragged batch: expected lens [seqs], starts [seqs + 1], positions and slots [tokens], got "
+                                              f"{[tuple(t.shape) for t in tensors]}")
+        object.__setattr__(self, "seqs", seqs)
+        object.__setattr__(self, "gpu", self.positions.get_device())
+        object.__setattr__(self, "args", (tokens, *(t.data_ptr() for t in tensors)))
 
 
 class CudaBackend:
@@ -376,14 +394,14 @@ class CudaBackend:
         """Reserve new_tokens[b] more slots per sequence; the step's layout goes into `batch`.  A step that does not fit
         changes nothing, describes no tokens and is reported by device_flush."""
         self._here("device_index_append", index.pages)
-        self._mine("device_index_append", torch.int32, new_tokens, batch.past_lens, batch.q_starts, batch.positions, batch.slots)
+        self._mine("device_index_append", torch.int32, new_tokens)
         seqs = index.desc.max_seqs
-        tokens = batch.positions.numel()
-        if new_tokens.shape != (seqs,) or batch.past_lens.numel() != seqs or batch.q_starts.numel() != seqs + 1 or batch.slots.numel() != tokens:
-            raise InfernoError(L.INF_E_SHAPE, f"device_index_append: the index has {seqs} sequences, got {tuple(new_tokens.shape)} lengths")
-        self._check(self._lib.inf_device_index_append(
-            self._ctx, C.byref(index.desc), new_tokens.data_ptr(), tokens, batch.past_lens.data_ptr(),
-            batch.q_starts.data_ptr(), batch.positions.data_ptr(), batch.slots.data_ptr()))
+        if new_tokens.shape != (seqs,) or batch.seqs != seqs:
+            raise InfernoError(L.INF_E_SHAPE, f"device_index_append: the index has {seqs} sequences, got {tuple(new_tokens.shape)} lengths "
+                                              f"and a batch of {batch.seqs}")
+        if batch.gpu != self.device.index:
+            raise InfernoError(L.INF_E_ARG, f"device_index_append: batch on {batch.positions.device}, the context is on {self.device}")
+        self._check(self._lib.inf_device_index_append(self._ctx, C.byref(index.desc), new_tokens.data_ptr(), *batch.args))
         return batch
 
     def device_index_truncate(self, index: DeviceIndex, keep_lens: torch.Tensor):

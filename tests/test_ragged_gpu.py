@@ -606,6 +606,13 @@ def test_refusals(be):
     refuses("ShapeMismatch", be.prepare_ragged_batch, 2, 0)
     batch = be.prepare_ragged_batch(2, 10)
     refuses("ShapeMismatch", be.device_index_append, index, ints(be, [1]), batch)
+    refuses("ShapeMismatch", be.device_index_append, index, ints(be, [1, 1]), be.prepare_ragged_batch(3, 10))
+    parts = (batch.past_lens, batch.q_starts, batch.positions, batch.slots)
+    refuses("ShapeMismatch", type(batch), *parts[:3], parts[3][:9])
+    refuses("ShapeMismatch", type(batch), parts[0], parts[1][:2], *parts[2:])
+    refuses("DType", type(batch), *parts[:3], parts[3].long())
+    refuses("Argument", type(batch), *parts[:3], torch.zeros((10, 2), dtype=torch.int32, device=be.device)[:, 0])
+    refuses("Argument", type(batch), *(t.cpu() for t in parts))
     refuses("DType", be.device_index_append, index, torch.ones(2, device=be.device), batch)
     refuses("ShapeMismatch", be.device_index_truncate, index, ints(be, [1, 1, 1]))
     wide = be.device_index(index.pages, index.lens, index.free_pages, index.free_count, 1 << 30)
