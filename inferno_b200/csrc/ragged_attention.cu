@@ -388,17 +388,19 @@ struct PageWalk {
 
 __device__ __forceinline__ bool few_rows(const RaggedParams& p, const Item& it) { return it.ntok <= p.few_tokens; }
 
-// ---- one tile of a stream: S in TMEM -> P over it, and the row's running maximum and sum.  A row of O is scaled only when
-// its maximum grew by more than 2^8: until then the weights stay below 2^8.  Each row decides for itself, so that its bits do
+// ---- one tile of a stream: S in TMEM -> P over it, and the row's running maximum and sum.  The maximum is kept as it comes out
+// of S and subtracted before the scale: rounded after the scale it is off by as much as half a step of itself, which the
+// exponents of large scores (2^28 and more) do not survive, and the row's top key must get a weight of 1.  A row of O is scaled
+// only when its maximum grew by more than 2^8 in weight: until then the weights stay below 2^8.  Each row decides for itself, so that its bits do
 // not depend on what else is in the warp.  The weights enter PV as fp16, half a step of 2^-11 each; their sum stays in 32 bits.
 
 // weights of 64 keys of a row, packed, and their sum
 __device__ __forceinline__ void exponentials(const uint32_t* x, float scale_log2, float m, uint32_t* packed, uint64_t* sums) {
-    const uint64_t scale2 = pack_f32x2(scale_log2, scale_log2), neg_m2 = pack_f32x2(-m, -m);
+    const uint64_t scale2 = pack_f32x2(scale_log2, scale_log2), neg_m2 = pack_f32x2(-m, -m);  // one rounding each, relative
 #pragma unroll
     for (int i = 0; i < 64; i += 2) {
         float a, b;
-        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, neg_m2), a, b);
+        unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), neg_m2), scale2), a, b);
         a = ex2_approx(a);
         b = ex2_approx(b);
         sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(a, b));
@@ -445,12 +447,12 @@ __device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, 
         tc_wait_ld64(x);
         top = fmaxf(top, max_of(x));
     }
-    const float m_new = fmaxf(m_used, top * p.scale_log2);  // the scale is positive
-    const bool grew = valid && m_new - m_used > RESCALE_THRESHOLD;
+    const float m_new = fmaxf(m_used, top), growth = (m_new - m_used) * p.scale_log2;  // the scale is positive
+    const bool grew = valid && growth > RESCALE_THRESHOLD;
     if (first) {
         m_used = m_new;
     } else if (__any_sync(0xffffffffu, grew)) {
-        const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
+        const float alpha = grew ? ex2_approx(-growth) : 1.0f;
         m_used = grew ? m_new : m_used;
         l *= alpha;
 #pragma unroll 1
@@ -508,13 +510,13 @@ __device__ __forceinline__ void softmax_tile_few(Shared& sh, const RaggedParams&
     float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float m_new = fmaxf(m_used, top * p.scale_log2);
+    const float m_new = fmaxf(m_used, top), growth = (m_new - m_used) * p.scale_log2;
     if (first) {
         m_used = m_new;
     } else {
-        const bool grew = valid && m_new - m_used > RESCALE_THRESHOLD;
+        const bool grew = valid && growth > RESCALE_THRESHOLD;
         if (__any_sync(0xffffffffu, grew)) {
-            const float alpha = grew ? ex2_approx(m_used - m_new) : 1.0f;
+            const float alpha = grew ? ex2_approx(-growth) : 1.0f;
             m_used = grew ? m_new : m_used;
             l *= alpha;
             uint32_t o[64];
@@ -535,8 +537,8 @@ __device__ __forceinline__ void softmax_tile_few(Shared& sh, const RaggedParams&
         uint32_t y[16];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float a = ex2_approx(fmaf(__uint_as_float(x[4 * (8 - half * 8 + k)]), p.scale_log2, -m_used));
-            const float b = ex2_approx(fmaf(__uint_as_float(x[4 * (8 - half * 8 + k) + 1]), p.scale_log2, -m_used));
+            const float a = ex2_approx((__uint_as_float(x[4 * (8 - half * 8 + k)]) - m_used) * p.scale_log2);
+            const float b = ex2_approx((__uint_as_float(x[4 * (8 - half * 8 + k) + 1]) - m_used) * p.scale_log2);
             sum += a + b;
             y[2 * k] = pack_half2(a, b);
             y[2 * k + 1] = 0u;  // lanes 8-15 hold no row
@@ -583,9 +585,9 @@ __device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& i
             return q < it.pieces ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + piece_row(it, q, 0, 0) + row_in_piece(mine))
                                  : make_float2(M_INIT, 0.f);
         };
-        auto merge = [](float& m, float& sum, float m2, float sum2) {
+        auto merge = [&](float& m, float& sum, float m2, float sum2) {
             const float top = fmaxf(m, m2);
-            sum = sum * ex2_approx(m - top) + sum2 * ex2_approx(m2 - top);
+            sum = sum * ex2_approx((m - top) * p.scale_log2) + sum2 * ex2_approx((m2 - top) * p.scale_log2);
             m = top;
         };
         const float gate = p.gate ? p.gate[out_mine] : 0.f;
@@ -620,7 +622,7 @@ __device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& i
                 }
                 gain = (p.gate ? softplus(gate) : 1.0f) / sum;
             }
-            const float w = ex2_approx(ml.x - m) * gain;  // 0 behind the last piece
+            const float w = ex2_approx((ml.x - m) * p.scale_log2) * gain;  // 0 behind the last piece
 #pragma unroll
             for (int e = 0; e < PIECES; ++e) {
                 if (q + e < it.pieces) {
@@ -1071,8 +1073,8 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     if (ok) ok = warp_wait(&sh.join[0], (uint32_t)joins & 1u);
                     tc_fence_after();
                     const float m1 = sh.ml[quarter * 32 + lane][0], m_all = fmaxf(m_used, m1);
-                    w0 = ex2_approx(m_used - m_all);
-                    w1 = ex2_approx(m1 - m_all);
+                    w0 = ex2_approx((m_used - m_all) * p.scale_log2);
+                    w1 = ex2_approx((m1 - m_all) * p.scale_log2);
                     l = l * w0 + sh.ml[quarter * 32 + lane][1] * w1;
                     m_used = m_all;
                 }

@@ -385,6 +385,29 @@ def test_attention_ragged_large_and_equal_scores(be):
     b.check(be)
 
 
+@pytest.mark.parametrize("past,new,Hq,Hkv,window", [
+    ([300, 0], [1, 2], 12, 2, 0),          # few rows
+    ([700, 40], [9, 1], 6, 1, 0),          # a light item
+    ([500], [20], 6, 1, 0),                # one stream of many rows
+    ([700], [64], 12, 2, 100),             # two streams, tiles that hide every key from some row
+    ([30000, 40], [2, 43], 6, 1, 0),       # items cut over many CTAs: the maxima meet in the join
+    ([9000], [130], 12, 2, 0),
+])
+@pytest.mark.parametrize("size,scale", [(2.0 ** 13, 0.0), (2.0 ** 10, 0.0), (1.0, 1e15), (2.0 ** 13, 1e8), (1.0, 1e-20)])
+@pytest.mark.parametrize("negative", [False, True])
+def test_attention_ragged_scores_of_any_size(be, past, new, Hq, Hkv, window, size, scale, negative):
+    """Queries and keys that are small whole numbers times a power of two: every sum of products is exact in 32 bits, so the
+    weights are known however large the scores are.  Equal scores differ by nothing, others by at least size^2 * scale, which
+    is rounded three times on its way into the exponent (3 * 2^-24 of it: below the tolerance where the weight is not 0)."""
+    b = Batch(be.device, past, new, Hq, Hkv, 16, seed=40, window=window)
+    b.q = (b.q * 1.2).round().clamp(-3, 3) * size
+    b.k = (b.k * 1.2).round().clamp(-3, 3) * size  # slots that no row sees stay NaN
+    if negative:
+        b.q, b.k = b.q.abs(), -b.k.abs()
+    for out_dtype in (torch.float16, torch.float32):
+        b.check(be, out_dtype=out_dtype, scale=scale)
+
+
 def test_attention_ragged_bad_page_and_bad_lengths_are_reported(be):
     from inferno_b200 import InfernoError
     b = Batch(be.device, [40, 100], [3, 2], 12, 2, 16, seed=6, filler=0.0)
