@@ -413,7 +413,7 @@ __device__ __forceinline__ void mask_scores(uint32_t col_s, int k0, int qpos, in
     for (int c = 0; c < BN; c += 32) {
         uint32_t x[32];
         tmem_ld32(col_s + c, x);
-        tc_wait_ld();
+        tc_wait_ld32(x);
 #pragma unroll
         for (int i = 0; i < 32; ++i)
             if (k0 + c + i > qpos || k0 + c + i < first_key) x[i] = 0xff800000u;  // -inf
@@ -459,7 +459,7 @@ __device__ __forceinline__ void softmax_tile(Shared& sh, const RaggedParams& p, 
         for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
             tmem_ld32(col_o + c * 32, o);
-            tc_wait_ld();
+            tc_wait_ld32(o);
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
             tmem_st32(col_o + c * 32, o);
@@ -521,7 +521,7 @@ __device__ __forceinline__ void softmax_tile_few(Shared& sh, const RaggedParams&
             l *= alpha;
             uint32_t o[64];
             tmem_ld_16x256(col_o, o);
-            tc_wait_ld();
+            tc_wait_ld64(o);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
                 o[4 * k] = __float_as_uint(__uint_as_float(o[4 * k]) * alpha);
@@ -1097,7 +1097,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                         uint32_t o[64];
                         float y[32];
                         tmem_ld_16x256(col_o, o);
-                        tc_wait_ld();
+                        tc_wait_ld64(o);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
                             y[2 * k] = __uint_as_float(o[4 * k]) * w0;
@@ -1105,7 +1105,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                         }
                         if (two) {
                             tmem_ld_16x256(col_o + D, o);
-                            tc_wait_ld();
+                            tc_wait_ld64(o);
 #pragma unroll
                             for (int k = 0; k < 16; ++k) {
                                 y[2 * k] = fmaf(__uint_as_float(o[4 * k]), w1, y[2 * k]);
@@ -1128,12 +1128,12 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                             uint32_t o[32];
                             float y[32];
                             tmem_ld32(col_o + c * 32, o);
-                            tc_wait_ld();
+                            tc_wait_ld32(o);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * w0;
                             if (two) {
                                 tmem_ld32(col_o + D + c * 32, o);
-                                tc_wait_ld();
+                                tc_wait_ld32(o);
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) y[i] = fmaf(__uint_as_float(o[i]), w1, y[i]);
                             }
