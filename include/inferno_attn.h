@@ -461,8 +461,9 @@ int32_t inf_linearize_paged(inf_ctx* ctx, const void* pool_f16, const inf_kv_poo
  * the host.  What the host cannot check is checked by the kernels and reported by inf_flush.
  * (The reference serves one sequence at a time and has no counterpart.) */
 
-/* inf_paged_index on the GPU: caller-owned int32 arrays.  Slots of `pages` below ceil(lens[b] / page_size) hold page ids;
- * the free list is a stack, free_pages[0 .. *free_count).  num_pages * page_size and max_pages * page_size must fit 31
+/* inf_paged_index on the GPU: caller-owned int32 arrays.  Slots of `pages` below ceil(lens[b] / page_size) hold page ids
+ * (also below a sliding window: there is no trim, and a row trimmed elsewhere cannot be cut or released here); the free
+ * list is a stack, free_pages[0 .. *free_count).  num_pages * page_size and max_pages * page_size must fit 31
  * bits, and max_seqs is at most 16384.  One call at a time may work on an index. */
 typedef struct inf_device_index {
     int32_t* pages;      /* [max_seqs][max_pages] */
@@ -478,13 +479,14 @@ int32_t inf_device_index_reset(inf_ctx* ctx, const inf_device_index* index);
  * that inf_gqa_attention_ragged takes), q_starts [max_seqs + 1] (first row of each sequence in the step's tensors; the
  * last entry is the number of rows), positions and slots [max_tokens] (slot = page id * page_size + offset; -1 in rows
  * behind the last token).  A step that does not fit -- more rows than max_tokens, a sequence longer than its table row,
- * more pages than are free -- is refused as a whole: the index stays as it is, the outputs describe a step without
- * tokens, and inf_flush reports it. */
+ * more pages than are free, an id outside the pool among the pages it takes or goes on filling -- is refused as a whole:
+ * the index stays as it is, the outputs describe a step without tokens, and inf_flush reports it. */
 int32_t inf_device_index_append(inf_ctx* ctx, const inf_device_index* index, const int32_t* new_tokens, int32_t max_tokens,
                                 int32_t* past_lens, int32_t* q_starts, int32_t* positions, int32_t* slots);
 /* Cuts sequence b to keep_lens[b] tokens (0 releases it, a negative value leaves it alone) and pushes its pages back, the
  * last sequence's last page first: a truncate to the lengths before an append restores the free list exactly.  A length
- * above the present one refuses the whole call (inf_flush). */
+ * above the present one, more pages than the pool has, or an id outside the pool among the pages that go back refuses the
+ * whole call: the index stays as it is (inf_flush). */
 int32_t inf_device_index_truncate(inf_ctx* ctx, const inf_device_index* index, const int32_t* keep_lens);
 
 /* inf_rope_append_gqa with a position and a slot per token: q [tokens][q_heads][128], k / v [tokens][kv_heads][128] in

@@ -10,8 +10,9 @@
 //
 // A cluster of up to sixteen CTAs shares a call.  Each takes the prefix sums over the whole batch into its own shared
 // memory, which is cheaper than waiting for another's, and then its share of the tokens and of the pages:
-// a search of the prefix sums gives the sequence, and a fresh page is read from the free list itself, not from the row
-// that another thread is writing.  The cluster's barrier stands between the last read of the lengths and their update.
+// a search of the prefix sums gives the sequence, and a fresh page is read from the free list itself.  Whether a page id is
+// none of the pool's is known behind those reads, to the CTA that met it; the CTAs tell each other, and the cluster's barrier
+// stands between the last read and the first write of the index, so that a refused call leaves all of it as it was.
 // An append and a truncate in a graph take 8.2 us for 32 decodes, 11.0 for 300 sequences of up to 9 new tokens, and 16.4
 // for 1000 of up to 127 (65 000 rows; eight CTAs 19.1, one alone 94), of which the two launches are about 5.
 #include "common.cuh"
@@ -38,6 +39,27 @@ __device__ __forceinline__ int cluster_rank() {
     int r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
+}
+
+// Whether `mine` holds for a thread of any of the cluster's CTAs (one cluster is the grid).  All threads call it, after a
+// cluster_arrive() of their own; everything they read before it has been read when it returns.
+__device__ __forceinline__ bool any_of_cluster(bool mine, int* s_flags) {
+    const bool here = __syncthreads_or(mine);
+    cluster_wait();  // the others run: their shared memory may be written
+    const int ctas = (int)gridDim.x;
+    if ((int)threadIdx.x < ctas) {
+        uint32_t there;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                     : "=r"(there)
+                     : "r"((uint32_t)__cvta_generic_to_shared(s_flags + cluster_rank())), "r"((int)threadIdx.x));
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(here ? 1 : 0) : "memory");
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    bool any = false;
+    for (int c = 0; c < ctas; ++c) any |= s_flags[c] != 0;
+    return any;
 }
 
 // Replaces x[0 .. n) by the sums of the values before them and writes the whole sum to x[n]; y likewise if given.  The
@@ -113,8 +135,10 @@ __global__ void __launch_bounds__(THREADS)
 device_index_append_kernel(IndexArgs a, const int* __restrict__ new_tokens, int max_tokens, int* __restrict__ past_lens,
                            int* __restrict__ q_starts, int* __restrict__ positions, int* __restrict__ slots) {
     __shared__ Sums s_warp[WARPS];
+    __shared__ int s_flags[MOST_CTAS];
     extern __shared__ int s_seqs[];
     int *s_past = s_seqs, *s_start = s_past + a.seqs, *s_fresh = s_start + a.seqs + 1;
+    cluster_arrive();
     inf_pdl_wait();
     inf_pdl_release();
     const int tid = threadIdx.x, rank = cluster_rank(), i0 = rank * THREADS + tid, stride = (int)gridDim.x * THREADS;
@@ -131,19 +155,23 @@ device_index_append_kernel(IndexArgs a, const int* __restrict__ new_tokens, int 
         s_fresh[b] = fits ? pages_of((long long)past + n, a.page_size) - pages_of(past, a.page_size) : 0;
     }
     const bool any_bad = __syncthreads_or(bad);
-    cluster_arrive();  // this CTA has read the lengths and the count
     const Sums total = prefix_sums(s_start, s_fresh, a.seqs, s_warp);
     if (total.x > max_tokens) bad |= INF_STATUS_BAD_LEN;
     if (total.y > free_count) bad |= INF_STATUS_NO_PAGES;
-    if (any_bad || total.x > max_tokens || total.y > free_count) {
-        if (bad && rank == 0) atomicOr(a.status, bad);
+    auto describe_no_tokens = [&] {
         for (int b = i0; b < a.seqs; b += stride) past_lens[b] = s_past[b];
         for (int b = i0; b <= a.seqs; b += stride) q_starts[b] = 0;
-        for (int t = i0; t < max_tokens; t += stride) positions[t] = slots[t] = -1;
+        for (long long t = i0; t < max_tokens; t += stride) positions[t] = slots[t] = -1;
+    };
+    if (any_bad || total.x > max_tokens || total.y > free_count) {
+        if (bad && rank == 0) atomicOr(a.status, bad);
+        describe_no_tokens();
         cluster_wait();
         return;
     }
-    // ---- every token's position and slot; rows behind the last token hold -1
+    // ---- every token's position and slot; rows behind the last token hold -1.  Every page that the step fills or takes has
+    // a token, so this meets all of their ids.
+    bool lost = false;
     const bool aligned = EACH == 4 && (((uintptr_t)positions | (uintptr_t)slots) & 15u) == 0;
     for (long long t0 = (long long)EACH * i0; t0 < max_tokens; t0 += (long long)EACH * stride) {
         int position[EACH], slot[EACH];
@@ -151,7 +179,6 @@ device_index_append_kernel(IndexArgs a, const int* __restrict__ new_tokens, int 
         for (int j = 0; j < EACH; ++j) position[j] = slot[j] = -1;
         if (t0 < total.x) {
             int b = holder_of(s_start, a.seqs, (int)t0), seen = -1, page = 0;
-            bool lost = false;
 #pragma unroll
             for (int j = 0; j < EACH; ++j) {
                 if (t0 + j >= total.x) break;
@@ -168,7 +195,6 @@ device_index_append_kernel(IndexArgs a, const int* __restrict__ new_tokens, int 
                 position[j] = at_token;
                 slot[j] = there ? page * a.page_size + at_token - at * a.page_size : -1;
             }
-            if (lost) atomicOr(a.status, INF_STATUS_BAD_PAGE);
         }
         if (aligned && t0 + EACH <= max_tokens) {
             *reinterpret_cast<int4*>(positions + t0) = make_int4(position[0], position[1 % EACH], position[2 % EACH], position[3 % EACH]);
@@ -179,6 +205,11 @@ device_index_append_kernel(IndexArgs a, const int* __restrict__ new_tokens, int 
                 if (t0 + j < max_tokens) positions[t0 + j] = position[j], slots[t0 + j] = slot[j];
         }
     }
+    if (any_of_cluster(lost, s_flags)) {  // (the barrier inside also orders the two stores to a row of the outputs)
+        if (i0 == 0) atomicOr(a.status, INF_STATUS_BAD_PAGE);
+        describe_no_tokens();
+        return;
+    }
     // ---- the fresh pages, and the batch's lengths and starts
     for (int f = i0; f < (int)total.y; f += stride) {
         const int b = holder_of(s_fresh, a.seqs, f);
@@ -186,18 +217,21 @@ device_index_append_kernel(IndexArgs a, const int* __restrict__ new_tokens, int 
     }
     for (int b = i0; b <= a.seqs; b += stride) {
         q_starts[b] = s_start[b];
-        if (b < a.seqs) past_lens[b] = s_past[b];
+        if (b < a.seqs) {
+            past_lens[b] = s_past[b];
+            a.lens[b] = s_past[b] + s_start[b + 1] - s_start[b];
+        }
     }
-    cluster_wait();
-    for (int b = i0; b < a.seqs; b += stride) a.lens[b] = s_past[b] + s_start[b + 1] - s_start[b];
     if (i0 == 0) *a.free_count = free_count - (int)total.y;
 }
 
 __global__ void __launch_bounds__(THREADS)
 device_index_truncate_kernel(IndexArgs a, const int* __restrict__ keep) {
     __shared__ Sums s_warp[WARPS];
+    __shared__ int s_flags[MOST_CTAS];
     extern __shared__ int s_seqs[];
     int *s_have = s_seqs, *s_hold = s_have + a.seqs, *s_gone = s_hold + a.seqs;  // from the last sequence to the first
+    cluster_arrive();
     inf_pdl_wait();
     inf_pdl_release();
     const int tid = threadIdx.x, rank = cluster_rank(), i0 = rank * THREADS + tid, stride = (int)gridDim.x * THREADS;
@@ -212,7 +246,6 @@ device_index_truncate_kernel(IndexArgs a, const int* __restrict__ keep) {
         s_gone[r] = k >= 0 && fits ? s_have[r] - pages_of(k, a.page_size) : 0;
     }
     const bool any_bad = __syncthreads_or(bad);
-    cluster_arrive();
     const Sums gone = prefix_sums(s_gone, nullptr, a.seqs, s_warp);
     const bool overfull = gone.x + free_count > a.num_pages;
     if (any_bad || overfull) {
@@ -221,13 +254,24 @@ device_index_truncate_kernel(IndexArgs a, const int* __restrict__ keep) {
         cluster_wait();
         return;
     }
-    for (int g = i0; g < (int)gone.x; g += stride) {
+    auto slot_of = [&](int g) {  // where the g-th page to be pushed stands
         const int r = holder_of(s_gone, a.seqs, g);
-        int* slot = a.pages + (long long)(a.seqs - 1 - r) * a.max_pages + s_have[r] - 1 - (g - s_gone[r]);
+        return a.pages + (long long)(a.seqs - 1 - r) * a.max_pages + s_have[r] - 1 - (g - s_gone[r]);
+    };
+    bool lost = false;
+    for (int g = i0; g < (int)gone.x; g += stride) {
+        const int page = *slot_of(g);
+        lost |= page < 0 || page >= a.num_pages;
+    }
+    if (any_of_cluster(lost, s_flags)) {
+        if (i0 == 0) atomicOr(a.status, INF_STATUS_BAD_PAGE);
+        return;
+    }
+    for (int g = i0; g < (int)gone.x; g += stride) {
+        int* slot = slot_of(g);
         a.free_pages[free_count + g] = *slot;
         *slot = -1;
     }
-    cluster_wait();
     for (int r = i0; r < a.seqs; r += stride)
         if (s_hold[r] >= 0) a.lens[a.seqs - 1 - r] = s_hold[r];
     if (i0 == 0) *a.free_count = free_count + (int)gone.x;

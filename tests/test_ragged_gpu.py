@@ -140,6 +140,70 @@ def test_a_step_that_does_not_fit_changes_nothing(be, new, max_tokens, why):
     assert (batch.positions == -1).all() and (batch.slots == -1).all()
 
 
+def _index_state(index):
+    """What an index holds: the table, the lengths, the stack and its count."""
+    return index.pages.clone(), index.lens.clone(), index.free_pages[:index.free_count.item()].clone(), index.free_count.clone()
+
+
+@pytest.mark.parametrize("seqs", [3, 9000])
+@pytest.mark.parametrize("bad", [-1, -2 ** 31, "pool", 2 ** 31 - 1])
+def test_pages_outside_the_pool_refuse_the_call(be, seqs, bad):
+    """A page id that is none, where a call takes, fills or gives back that page: it is reported and nothing changes.  The bad
+    one stands with the last sequence, which another of the cluster's CTAs may hold than the first ones."""
+    from inferno_b200 import InfernoError
+    P, last = 16, seqs - 1
+    num_pages = 3 * seqs + 4
+    bad = num_pages if bad == "pool" else bad
+    index = be.prepare_device_index(num_pages, P, seqs, 4)
+    max_tokens = 40 * seqs
+    batch = be.prepare_ragged_batch(seqs, max_tokens)
+    be.device_index_append(index, ints(be, [20] * seqs), batch)  # two pages each, the second one partly filled
+    be.device_flush()
+
+    def refused(call):
+        before = _index_state(index)
+        call()
+        with pytest.raises(InfernoError, match="page id"):
+            be.device_flush()
+        for was, now in zip(before, _index_state(index)):
+            assert torch.equal(was, now)
+
+    def refused_step(new):
+        refused(lambda: be.device_index_append(index, new, batch))
+        assert (batch.q_starts == 0).all() and (batch.positions == -1).all() and (batch.slots == -1).all()
+        assert torch.equal(batch.past_lens, index.lens)
+
+    step = ints(be, [1] * last + [30])  # two more pages for the last sequence, none for the others
+    # a page that would be given back
+    good = index.pages[last].clone()
+    for slot in (0, 1):
+        index.pages[last, slot] = bad
+        refused(lambda: be.device_index_truncate(index, torch.zeros_like(index.lens)))
+        index.pages[last] = good
+    # a page that the step would go on filling
+    index.pages[last, 1] = bad
+    refused_step(step)
+    index.pages[last] = good
+    # a page that the step would take
+    top = index.free_count.item() - 1
+    for at in (top, top - 1):
+        kept = index.free_pages[at].item()
+        index.free_pages[at] = bad
+        refused_step(step)
+        index.free_pages[at] = kept
+    # pages that no call touches may hold anything: a full one, a slot behind the length, an entry further down the stack
+    index.pages[last, 0] = bad
+    index.pages[0, 3] = bad
+    index.free_pages[0] = bad
+    be.device_index_append(index, step, batch)
+    be.device_index_truncate(index, batch.past_lens)
+    be.device_flush()
+    index.pages[last, 0] = good[0]
+    be.device_index_truncate(index, torch.zeros_like(index.lens))
+    be.device_flush()
+    assert index.free_count.item() == num_pages and (index.lens == 0).all()
+
+
 # ------------------------------------------------------------------------------------------------ rope + append
 @pytest.mark.parametrize("T,pad,Hq,Hkv,rotary,norm,dtype,fused,P,far", [
     (1, 0, 48, 8, 64, True, torch.float16, False, 16, 100),
