@@ -680,6 +680,7 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         mbar_init(&sh.drained, 1);
         mbar_init(&sh.part_bar, 8);
         mbar_init(&sh.flag_bar, 1);
+        sh.last_piece[0] = sh.last_piece[1] = 0;
         mbar_fence_init();
     }
     if (warp == 9) {
@@ -1182,7 +1183,8 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             if (tid == 0) mbar_arrive(&sh.flag_bar);
             if (ok) ok = warp_wait(&sh.flag_bar, 0);
             const bool one = sh.last_piece[0], other = pieces == 2 && sh.last_piece[1], both = one && other;
-            if (one || other)  // half of the warps each where there are two
+            // half of the warps each where there are two; none behind a wait that gave up, whose items may never have been written
+            if (ok && (one || other))
                 join_pieces(p, sh.piece[both ? warp >> 2 : (one ? 0 : 1)], both ? warp & 3 : warp, both ? 4 : 8, lane);
         }
         if (!ok && lane == 0) atomicOr(p.status, INF_STATUS_WAIT_TIMEOUT);
