@@ -1243,12 +1243,15 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
             return inf_fail(ctx, INF_E_DTYPE, "%s: output dtype must be f32 or f16", what);
         int rc = inf_validate_table(ctx, table, pool->num_pages, pool->page_size, 0, what, sliding_window, 0);
         if (rc != INF_OK) return rc;
+        RaggedParams p{};
+        const int grid = ctx->sm_count;
+        rc = ragged_scratch(ctx, grid, &p.part_acc, &p.part_ml, &p.counters);  // also of a call without tokens, which may be the first
+        if (rc != INF_OK) return rc;
         if (tokens == 0) return INF_OK;
         if (!q_f16 || !q_starts || !out) return inf_fail(ctx, INF_E_ARG, "%s: null pointer", what);
         if (((uintptr_t)q_f16 | (uintptr_t)out | (uintptr_t)pool->k | (uintptr_t)pool->v) & 15u)
             return inf_fail(ctx, INF_E_ARG, "%s: tensors must be 16-byte aligned", what);
         const int group = q_heads / pool->kv_heads;
-        RaggedParams p{};
         p.q = (const __half*)q_f16;
         p.pages = table->pages;
         p.lens = table->lens;
@@ -1273,9 +1276,6 @@ extern "C" int32_t inf_gqa_attention_ragged(inf_ctx* ctx, const void* q_f16, con
         p.out_f16 = out_dtype == INF_DTYPE_F16;
         p.out_sectors = ((uintptr_t)out & 31u) == 0;
         p.status = ctx->status;
-        const int grid = ctx->sm_count;
-        rc = ragged_scratch(ctx, grid, &p.part_acc, &p.part_ml, &p.counters);
-        if (rc != INF_OK) return rc;
         CUtensorMap tq, tq_light, tk, tv;
         {
             const uint64_t dims[3] = {D, (uint64_t)q_heads, (uint64_t)tokens}, strides[2] = {D * 2, (uint64_t)q_heads * D * 2};

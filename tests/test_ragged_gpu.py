@@ -589,6 +589,22 @@ def test_captured_steps_replay_with_other_lengths(be):
     _run_steps(be, s, graph.replay, seed=2)
 
 
+def test_a_first_call_without_tokens_is_enough_before_a_capture(be):
+    """The context's first call allocates the scratch, whatever its step holds, so that the next one can be captured."""
+    from inferno_b200 import CudaBackend
+    b = Batch(be.device, [9000], [130], 12, 2, 16, seed=41)
+    want = b.check(be)
+    torch.cuda.synchronize()
+    own = CudaBackend(0, stream=torch.cuda.Stream())
+    pool, table, out = own.kv_pool(b.k, b.v), own.page_table(b.pages, b.past_lens, validate_on_host=False), torch.zeros_like(b.q)
+    own.gqa_attention_ragged(b.q[:0], pool, table, ints(be, [0, 0]))
+    graph = own.capture_graph(lambda: own.gqa_attention_ragged(b.q, pool, table, b.q_starts, out=out), warmup=0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[:b.rows], want[:b.rows])
+    own.close()
+
+
 def test_two_graphs_of_one_context_share_its_scratch(be):
     """Two captured attentions, both with items cut over many CTAs, replayed in turn and twice in a row, with an eager call
     between: each gives the bits of its own eager call."""
