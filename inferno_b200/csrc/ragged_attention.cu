@@ -573,7 +573,6 @@ __device__ __forceinline__ long long piece_row(const Item& it, int q, int st, in
 // time: the time is latency, so what counts is how many loads are under way.
 __device__ __forceinline__ void join_pieces(const RaggedParams& p, const Item& it, int warp, int warps, int lane) {
     constexpr int ROWS = 8, PIECES = 4;
-    __threadfence();
     const int per = p.stream_tokens * p.group, all = it.ntok * p.group;  // rows of a full stream, of the item
     auto row_in_piece = [&](int rr) { return rr < per ? rr : BM + rr - per; };
 #pragma unroll 1
@@ -1169,13 +1168,16 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         }
         // ---- cut items (the part's first and last at most): whoever finishes the last piece joins them in the order of the keys
         if (pieces > 0) {
-            __threadfence();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.part_bar);
             if (ok) ok = warp_wait(&sh.part_bar, 0);
             if (tid < pieces) {
                 const Item& mine = sh.piece[tid];
+                // One thread counts for its CTA: the pieces that a barrier has shown to it before the count, and the others' pieces
+                // behind it, which a barrier shows to the warps that join.
+                __threadfence();
                 const int before = atomicAdd(&p.counters[mine.group], 1);
+                __threadfence();
                 sh.last_piece[tid] = before + 1 == mine.pieces;
                 if (before + 1 == mine.pieces) p.counters[mine.group] = 0;  // for the next launch
             }
