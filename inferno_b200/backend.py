@@ -382,6 +382,7 @@ class CudaBackend:
                                          free_pages.numel(), page_size, pages.shape[0], pages.shape[1]))
 
     def device_index_reset(self, index: DeviceIndex):
+        self._here("device_index_reset", index.pages)
         self._check(self._lib.inf_device_index_reset(self._ctx, C.byref(index.desc)))
 
     def prepare_ragged_batch(self, max_seqs: int, max_tokens: int) -> RaggedBatch:

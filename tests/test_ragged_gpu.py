@@ -204,6 +204,19 @@ def test_pages_outside_the_pool_refuse_the_call(be, seqs, bad):
     assert index.free_count.item() == num_pages and (index.lens == 0).all()
 
 
+def test_index_calls_refuse_an_index_elsewhere(be):
+    """Tensors that are not on the context's GPU reach no kernel, whichever call gets the index first."""
+    from inferno_b200 import InfernoError
+    from inferno_b200.backend import DeviceIndex
+    index = be.prepare_device_index(8, 16, 2, 4)
+    away = DeviceIndex(index.pages.cpu(), index.lens.cpu(), index.free_pages.cpu(), index.free_count.cpu(), index.desc)
+    for call in (lambda: be.device_index_reset(away), lambda: be.device_index_truncate(away, ints(be, [0, 0])),
+                 lambda: be.device_index_append(away, ints(be, [1, 1]), be.prepare_ragged_batch(2, 4))):
+        with pytest.raises(InfernoError) as e:
+            call()
+        assert e.value.kind == "Argument"
+
+
 # ------------------------------------------------------------------------------------------------ rope + append
 @pytest.mark.parametrize("T,pad,Hq,Hkv,rotary,norm,dtype,fused,P,far", [
     (1, 0, 48, 8, 64, True, torch.float16, False, 16, 100),
