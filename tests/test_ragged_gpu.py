@@ -264,6 +264,32 @@ def test_rope_append_ragged(be, T, pad, Hq, Hkv, rotary, norm, dtype, fused, P, 
         assert (p.transpose(1, 2).reshape(pages * P, Hkv, 128)[unused] == filler).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rotary,norm", [(0, ""), (64, "q"), (64, "k"), (128, "q"), (128, "k")])
+def test_rope_append_ragged_without_a_table_or_with_one_norm(be, dtype, rotary, norm):
+    """Without a table rows are stored as they are; a norm weight for one of the two leaves the other its size."""
+    T, Hq, Hkv, P = 21, 12, 4, 16
+    g = torch.Generator(device=be.device).manual_seed(44)
+    q, k, v = (torch.randn((T, h, 128), generator=g, device=be.device).to(dtype) for h in (Hq, Hkv, Hkv))
+    qw, kw = (1 + 0.2 * torch.randn(128, generator=g, device=be.device) if norm == x else None for x in "qk")
+    slots = torch.randperm(3 * P, generator=g, device=be.device)[:T].to(torch.int32)
+    positions = torch.randint(0, 5000, (T,), generator=g, device=be.device, dtype=torch.int32)
+    pool = be.prepare_kv_pool(3, P, Hkv)
+    inv = (1 / 10000.0 ** (torch.arange(0, rotary, 2, dtype=torch.float64) / max(1, rotary))).float()
+    rope = be.prepare_rope_table(inv, rotary, 1.0) if rotary else None
+    out = be.rope_append_gqa_ragged(q, k, v, rope, pool, positions, slots, q_norm=qw, k_norm=kw)
+    be.device_flush()
+    slot = slots.long()
+    stored = pool.k[slot // P, :, slot % P]
+    assert torch.equal(pool.v[slot // P, :, slot % P], v.half())
+    if not rotary:
+        assert torch.equal(out, q.half()) and torch.equal(stored, k.half())
+        return
+    inv = inv.to(be.device)
+    assert_rows_close(out, rope_reference(q, qw, 1e-6, positions, inv, rotary), "q")
+    assert_rows_close(stored, rope_reference(k, kw, 1e-6, positions, inv, rotary), "k")
+
+
 def test_rope_append_ragged_agrees_with_the_uniform_call(be):
     """One token count for all sequences: the same rows as rope_append_gqa, the rotation aside, whose angle is taken in 64
     bits here: at positions below 2048 the two angles differ by 2^-14 at most, the rows by that times their size."""
@@ -523,6 +549,43 @@ def test_attention_ragged_equals_the_uniform_prefill_and_decode(be):
     old = be.gqa_prefill_paged(b.q.view(B, T, Hq, 128), pool, table, out_dtype=torch.float32)
     be.device_flush()
     assert (got - old.view(got.shape)).abs().max() <= 2 * (2.0 ** -11 + 2.0 ** -14) * b.v.abs().max()
+
+
+@pytest.mark.parametrize("past,Hq,Hkv,P,window", [
+    ([0, 15, 127, 128, 700], 48, 8, 16, 0),
+    ([3000, 1, 511], 12, 2, 64, 512),
+    ([20000, 40], 64, 8, 16, 0),
+    ([90, 5000], 8, 8, 32, 100),
+])
+@pytest.mark.parametrize("gate", [False, True])
+def test_attention_ragged_of_one_token_each_equals_the_uniform_decode(be, past, Hq, Hkv, P, window, gate):
+    """Both calls are within one tolerance of the exact value (assert_attention_close, 32-bit output), so within two of each
+    other.  The uniform call takes the gate as log(1 + e^g), whose sum is off by 2^-24 and the logarithm by as much:
+    2^-23 of the ungated row, and what is left of the two gates' roundings counts as often again."""
+    from tests.ragged import attention_reference
+    n = len(past)
+    b = Batch(be.device, past, [1] * n, Hq, Hkv, P, seed=42, window=window, filler=0.0)
+    pool, g = be.kv_pool(b.k, b.v), b.gate if gate else None
+    got = be.gqa_attention_ragged(b.q, pool, be.page_table(b.pages, b.past_lens), b.q_starts, sliding_window=window, gate=g, out_dtype=torch.float32)
+    old = be.gqa_decode_paged(b.q, pool, be.page_table(b.pages, b.past_lens + 1), max(past) + 1, sliding_window=window, gate=g, out_dtype=torch.float32)
+    be.device_flush()
+    _, size = attention_reference(b.q, b.k, b.v, b.pages, past, [1] * n, window, g)
+    _, ungated = attention_reference(b.q, b.k, b.v, b.pages, past, [1] * n, window)
+    tol = 2 * ((2.0 ** -11 + 2.0 ** -14 + 2.0 ** -24) * size + (b.keys * 2.0 ** -25 + 1e-7) * size.amax(-1, keepdim=True)) + 2.0 ** -22 * ungated
+    err = (got.double() - old.double()).abs()
+    assert (err <= tol).all(), f"worst {float((err / tol).max()):.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("filler", [float("nan"), float("inf"), 6e4])
+def test_attention_ragged_rows_behind_the_last_sequence_may_hold_anything(be, filler):
+    """A batch padded to the size of a captured step: queries and gates of the padding enter tiles with real rows and
+    change none of their bits."""
+    for past, new, Hq, Hkv in (([300, 40], [1, 2], 12, 2), ([700], [9], 6, 1), ([500], [20], 6, 1), ([700, 9000], [64, 30], 12, 2)):
+        b = Batch(be.device, past, new, Hq, Hkv, 16, seed=43, spare_rows=70)
+        want = b.check(be, gate=True)
+        b.q[b.rows:] = filler
+        b.gate[b.rows:] = filler
+        assert torch.equal(b.check(be, gate=True), want)
 
 
 # ------------------------------------------------------------------------------------------------ the step
