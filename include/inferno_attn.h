@@ -493,7 +493,8 @@ int32_t inf_device_index_truncate(inf_ctx* ctx, const inf_device_index* index, c
  * in_dtype, heads contiguous, tokens q_stride / k_stride / v_stride elements apart (parts of one projection's rows need
  * no copy).  q_out_f16 [tokens][q_heads][128] receives the roped queries.  Rows with a negative position are padding and
  * touch nothing.  A slot outside the pool is reported and its key and value dropped; slots of one call must differ.
- * Angles are exact for every 31-bit position.  Without a rope table rows are stored as they are (no norm either). */
+ * Angles are reduced in 64 bits: off by less than 2^-20 at any 31-bit position (frequencies up to 1).  Without a rope
+ * table rows are stored as they are (no norm either). */
 int32_t inf_rope_append_gqa_ragged(inf_ctx* ctx, const void* q, const void* k, const void* v, int64_t q_stride,
                                    int64_t k_stride, int64_t v_stride, int32_t in_dtype, const float* q_norm_weight,
                                    const float* k_norm_weight, float eps, const inf_rope_table* rope,
@@ -506,7 +507,9 @@ int32_t inf_rope_append_gqa_ragged(inf_ctx* ctx, const void* q, const void* k, c
  * p = lens[b] + t.  gate f32 [tokens][q_heads] (optional) applies softplus(gate); scale <= 0 means 1/sqrt(128); out
  * [tokens][q_heads][128] in out_dtype.  Rows from q_starts[batch] on are left as they were.  Up to 128 query heads per KV
  * head (INF_UNSUPPORTED beyond) and 2^29 tokens in a row of the page table.  A sequence whose rows or length do not fit is
- * skipped and reported, a page id outside the pool is reported and its keys read as zeros.  Keys and values that some row of
+ * skipped and reported, a page id outside the pool is reported and its keys read as zeros.  Scores may be of any size that
+ * finite queries and keys give, scale at most 1e15.  Where the keys of a sequence are divided depends on the batch, and so do the
+ * last bits of its rows; the same batch gives the same bits.  Keys and values that some row of
  * the call sees must be finite: one that is not may reach other rows of its sequence.  Pool slots that no row sees, behind a
  * sequence's last token and below its first row's window, may hold anything; pages wholly below that window may have been
  * given back.  The context's first call allocates scratch (about 40 MB); make it before a capture.  Calls of one context, and

@@ -13,8 +13,9 @@
 // a search of the prefix sums gives the sequence, and a fresh page is read from the free list itself.  Whether a page id is
 // none of the pool's is known behind those reads, to the CTA that met it; the CTAs tell each other, and the cluster's barrier
 // stands between the last read and the first write of the index, so that a refused call leaves all of it as it was.
-// An append and a truncate in a graph take 8.2 us for 32 decodes, 11.0 for 300 sequences of up to 9 new tokens, and 16.4
-// for 1000 of up to 127 (65 000 rows; eight CTAs 19.1, one alone 94), of which the two launches are about 5.
+// An append and a truncate in a graph take 9.1 us for 32 decodes, 11.0 for 300 sequences of up to 9 new tokens, and 18.2
+// for 1000 of up to 127 (65 000 rows), of which the two launches are about 5.  Without the check of the page ids, whose
+// barrier and second search stand in the chain, it was 8.2, 9.4 and 15.9 (with eight CTAs 19.1 for the last, with one 94).
 #include "common.cuh"
 
 namespace {

@@ -36,11 +36,12 @@
 //
 // What bounds it, and what it takes on a B200 (a floor is the keys' bytes at the measured copy bandwidth or the products at the
 // measured cuBLAS rate; the first figure from a cool GPU, the second held at its power limit):
-//   32 decodes of 1 024-16 384 keys, 48 / 8 heads   125, 130 us   floor 114: memory
-//   24 sequences of 6 drafts, 64 / 8 heads           80, 82        60: memory, then the CTAs' start (5 us), unequal SMs, the join
-//   46 decodes and two chunks of 1 024, 48 / 8      148, 170       84: the chunks' tiles (softmax and MMAs in turn), joins
-//   40 decodes and a chunk of 777, window 512        50, 50        10: five tiles an item, so its start and end; no two parts alike
-//   a chunk of 4 096 on 8 192 keys, 48 / 8          935, 1 030    626: a stream's tile takes softmax 2 100 + MMAs 1 300 cycles,
+//   32 decodes of 1 024-16 384 keys, 48 / 8 heads   125, 131 us   floor 114: memory
+//   24 sequences of 6 drafts, 64 / 8 heads           79, 83        60: memory, then the CTAs' start (5 us), unequal SMs, the join
+//   46 decodes and two chunks of 1 024, 48 / 8      151, 173       84: the chunks' tiles (softmax and MMAs in turn), joins
+//   40 decodes and a chunk of 777, window 512        51, 51        10: five tiles an item, so its start and end; the largest part is
+//                                                                  worth 1.5 times the mean
+//   a chunk of 4 096 on 8 192 keys, 48 / 8          945, 1 040    626: a stream's tile takes softmax 2 100 + MMAs 1 300 cycles,
 //                                                                  and the other stream covers half of that
 //   one decode of 100 keys                             9 in a graph: launch, cold code, a chain of five waits
 #include <cuda_fp16.h>
@@ -390,8 +391,9 @@ __device__ __forceinline__ bool few_rows(const RaggedParams& p, const Item& it) 
 
 // ---- one tile of a stream: S in TMEM -> P over it, and the row's running maximum and sum.  The maximum is kept as it comes out
 // of S and subtracted before the scale: rounded after the scale it is off by as much as half a step of itself, which the
-// exponents of large scores (2^28 and more) do not survive, and the row's top key must get a weight of 1.  A row of O is scaled
-// only when its maximum grew by more than 2^8 in weight: until then the weights stay below 2^8.  Each row decides for itself, so that its bits do
+// exponents of large scores (2^28 and more) do not survive, and the row's top key must get a weight of 1 (one instruction more
+// for two keys: the chunk of 4 096 took 912 us before).  A row of O is scaled only when its maximum grew by more than 2^8 in
+// weight: until then the weights stay below 2^8.  Each row decides for itself, so that its bits do
 // not depend on what else is in the warp.  The weights enter PV as fp16, half a step of 2^-11 each; their sum stays in 32 bits.
 
 // weights of 64 keys of a row, packed, and their sum
@@ -832,8 +834,9 @@ ragged_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 for (int t = max(0, tiles - VS); t < tiles; ++t) warp_wait(&sh.v_full[t % VS], (uint32_t)(t / VS) & 1u);
         } else if (warp == 11) {
             // ------------------------------------------------ Q: a stream's tile is free when its last S has retired.  An item of
-            // few or light rows finds zeros in the tile's other rows: the tensor cores work on all 128, and what they draw for
-            // multiplying by zero leaves the clock higher when the GPU is at its power limit.
+            // few rows finds zeros in the tile's other rows, a light one in the upper 64 (below them its box may bring the next
+            // tokens' rows and leave older ones, which nothing reads the products of): the tensor cores work on all 128, and what
+            // they draw for multiplying by zero leaves the clock higher when the GPU is at its power limit.
             int uses0 = 0, uses1 = 0;
             int held = 0;  // rows of stream 0's tile that are not zero: of an item of few rows, or -1: light, -2: any
             auto few_row = [](int r) { return (r & 3) * 16 + (r >> 2); };  // row r of few lies there

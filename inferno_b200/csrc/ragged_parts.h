@@ -10,7 +10,7 @@
 
 constexpr int RAGGED_TILE = 128;  // keys of a tile
 // Costs, in halves of a key of a light item.  A key of an item of two streams costs two and a half times as much (with twice:
-// two chunks of 1 024 among 46 decodes 159 us instead of 148, a window of 512 49 instead of 51), of one stream of many rows one
+// two chunks of 1 024 among 46 decodes 158 us instead of 151, a window of 512 50 instead of 51.5), of one stream of many rows one
 // and a half times (items of 33 to 64 rows count as light: 24 sequences' drafts 95 us as heavy ones, 82 as light); an item
 // costs some keys besides (256 light ones; with 192 or 384 the window takes 54 us).  A CTA's part is worth a tile of two
 // streams at least, which keeps two cuts of one item from falling on the same tile, and no more, so that short decodes are
